@@ -502,7 +502,7 @@ def _run_pages(s):
     s["tables"].copy_(s["tables0"])
     s["refs"].copy_(s["refs0"])
     if own:
-        s["pool"].compact(s["cache"], s["tables"], s["lens"])
+        s["pool"].compact(s["cache"], s["tables"])
     else:
         _plain_compact(s)
     return {"tables": s["tables"], "refs": s["refs"], **_codes(s)}
