@@ -336,6 +336,113 @@ int rth_rmsnorm_bf16(uint16_t* y, const uint16_t* x, const uint16_t* g, int num_
  * counterpart: lets a checker restate the summation order. */
 int rth_rmsnorm_lanes(int hidden_dim);
 
+/* ---- a batch of sequences (no counterparts in the reference, which serves one
+ * sequence at a time) -------------------------------------------------------
+ *
+ * Packed rows: the tokens of num_seqs sequences one behind the other; sequence
+ * b holds rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (cu_seqlens: num_seqs + 1
+ * device ints, ascending; bounds past num_rows are taken as num_rows). Rows
+ * behind the last sequence are neither read nor written. Row strides are in
+ * elements, multiples of 8, at least heads * head_dim (so q, k and v may be
+ * slices of one projection's rows). Rows of q, k, v and out start 16-byte aligned.
+ *
+ * Block tables of a batch: [num_seqs, table_blocks] device ints; entry i of row
+ * b is the page of positions i * block_size .. (i + 1) * block_size - 1 of
+ * sequence b, an entry outside 0 .. num_blocks - 1 names no page. Slabs hold
+ * num_blocks pages of block_size positions (a power of two >= 32). num_seqs <=
+ * 4096. */
+
+/* Causal attention over whole prompts: row t of sequence b attends rows
+ * cu_seqlens[b] .. t, straight from the bf16 k and v ([rows, Hkv, D], no
+ * cache). head_dim 64, 128, 256; any Hq / Hkv. out may not overlap the inputs.
+ * A key that a row does not see leaves no trace in it, whatever k and v hold there. */
+int rth_attn_packed(uint16_t* out, const uint16_t* q, const uint16_t* k, const uint16_t* v,
+                    const int* cu_seqlens, int num_seqs, int num_rows, int64_t out_stride,
+                    int64_t q_stride, int64_t k_stride, int64_t v_stride, int num_q_heads,
+                    int num_kv_heads, int head_dim, float scale, void* stream);
+
+/* Appends a batch's K and V rows ([rows, Hkv, D] bf16, packed; cu_seqlens NULL:
+ * one row per sequence, row b of sequence b) to the sequences' pages: row t of
+ * sequence b at position at_pos[b] + t - cu_seqlens[b] of it, byte for byte
+ * as rth_kv_append_fp8_paged would. A row whose position lies outside the table, or
+ * whose table entry names no page, is not stored. head_dim % 8 == 0, 8 <=
+ * head_dim <= 512. */
+int rth_kv_append_fp8_batch(uint8_t* k_cache, uint8_t* v_cache, float* k_scale, float* v_scale,
+                            const uint16_t* k, const uint16_t* v, int64_t k_stride,
+                            int64_t v_stride, const int* cu_seqlens, const int* at_pos,
+                            int num_seqs, int num_rows, int num_kv_heads, int head_dim,
+                            const int* block_tables, int table_blocks, int num_blocks,
+                            int block_size, void* stream);
+
+/* Decode attention of a batch, one query token per sequence (q, out [num_seqs,
+ * Hq, D]): sequence b attends keys 0 .. lens[b] - 1. The first *prefix_len of
+ * them are the same for every sequence and lie in the pages of prefix_table
+ * [prefix_blocks]: they are read and multiplied once for the whole batch. The
+ * others lie in the sequence's own row of block_tables, at their own positions
+ * (so tables that rth_pages_fork made can be passed whole, with any one of
+ * their rows as prefix_table). prefix_table and prefix_len NULL: nothing is shared. lens[b] <= 0:
+ * an unused slot, its output row is zeros. Keys past a table's end, and keys whose
+ * table entry names no page, are left out. head_dim 64, 128, 256; any Hq / Hkv.
+ * partial: rth_batch_scratch_floats floats, 16-byte aligned, no
+ * initialization needed, not shared by calls that overlap (graphs included). */
+size_t rth_batch_scratch_floats(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim);
+int rth_attn_decode_batch(uint16_t* out, int64_t out_stride, const uint16_t* q, int64_t q_stride,
+                          const uint8_t* k, const uint8_t* v, const float* k_scale,
+                          const float* v_scale, const int* block_tables, int table_blocks,
+                          int num_blocks, int block_size, const int* lens,
+                          const int* prefix_table, int prefix_blocks, const int* prefix_len,
+                          float* partial, int num_seqs, int num_q_heads, int num_kv_heads,
+                          int head_dim, float scale, void* stream);
+
+/* Pages of a paged cache of num_layers layers (slabs [num_layers, num_blocks *
+ * block_size, Hkv, D] and [.., Hkv]; head_dim % 8 == 0), with the bookkeeping on the device: refs
+ * [num_blocks] counts the table entries that hold each page, a page with refs
+ * <= 0 is free, and the lowest free pages are given out first. A table entry < 0
+ * holds no page. `work` is scratch of rth_pages_work_ints ints (no
+ * initialization needed, not shared by calls that overlap); *status gets bit 0
+ * when the free pages did not suffice and bit 1 when a table is too short, and the call has
+ * then changed nothing else. Calls on one pool run one behind the other (one
+ * stream, or ordered streams). */
+size_t rth_pages_work_ints(int num_blocks);
+
+/* Copies page src[i] to page dst[i] in every layer, i < count. The dst pages are
+ * distinct, and none of them is a src page; ids that name no page are skipped. */
+int rth_pages_copy(uint8_t* k, uint8_t* v, float* k_scale, float* v_scale, int num_layers,
+                   int num_blocks, int block_size, int num_kv_heads, int head_dim,
+                   const int* src, const int* dst, int count, void* stream);
+
+/* Gives sequence b the pages it lacks for positions lens[b] .. lens[b] +
+ * n_new[b] - 1 (entries of its table row that are < 0), in order of b. */
+int rth_pages_reserve(int* refs, int* work, int* status, int num_blocks, int block_size,
+                      int* block_tables, int table_blocks, const int* lens, const int* n_new,
+                      int num_seqs, void* stream);
+
+/* Child i becomes a copy of sequence parents[i] of the source tables: it shares
+ * the parent's filled pages (refs + 1) and gets, where the last one is part
+ * filled, a page of its own with a copy of the filled rows of every layer.
+ * dst_tables [num_children, table_blocks] and dst_lens are written whole and
+ * may not overlap the source's; what they held before is to be freed first. A
+ * parent outside 0 .. num_src - 1 gives an empty child. num_children <=
+ * min(4096, num_blocks). */
+int rth_pages_fork(uint8_t* k, uint8_t* v, float* k_scale, float* v_scale, int num_layers,
+                   int num_blocks, int block_size, int num_kv_heads, int head_dim, int* refs,
+                   int* work, int* status, int* dst_tables, int* dst_lens,
+                   const int* src_tables, const int* src_lens, int table_blocks, int num_src,
+                   const int* parents, int num_children, void* stream);
+
+/* Frees the sequences with drop[b] != 0 (drop NULL: all): refs - 1 for each
+ * page of their rows, entries -1, lengths 0. */
+int rth_pages_free(int* refs, int num_blocks, int* block_tables, int table_blocks, int* lens,
+                   const int* drop, int num_seqs, void* stream);
+
+/* Moves the pages in use down to 0 .. (their number) - 1: those above, lowest
+ * first, into the free ones below, lowest first, in every layer; the tables
+ * (all that hold pages of the pool) and refs follow. */
+int rth_pages_compact(uint8_t* k, uint8_t* v, float* k_scale, float* v_scale, int num_layers,
+                      int num_blocks, int block_size, int num_kv_heads, int head_dim, int* refs,
+                      int* work, int* block_tables, int table_blocks, int num_seqs,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

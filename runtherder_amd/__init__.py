@@ -12,13 +12,17 @@ from .ops import (  # noqa: F401
     AttentionBackend,
     AttnConfig,
     BackendKind,
+    BatchAttention,
+    KVBatchView,
     KVCache,
     KVSlabs,
     KVView,
     NaiveAttention,
     PagedKVCache,
+    PagePool,
     advance_position,
     attention_causal_bf16,
+    batch_scratch_floats,
     DECODE_MFMA,
     DECODE_VALU,
     decode_path,
@@ -27,12 +31,15 @@ from .ops import (  # noqa: F401
     flash_decode_append_split_bf16,
     flash_decode_rope_append_split_bf16,
     flash_decode_qk_norm_rope_append_split_bf16,
+    flash_decode_batch_bf16,
     flash_decode_split_bf16,
     flash_decode_split_bf16_noalloc,
+    flash_packed_bf16,
     flash_prefill_bf16,
     flash_prefill_split_bf16,
     PREFILL_SPLIT_MAX_TOKENS,
     flash_split_scratch_floats,
+    kv_append_fp8_batch,
     make_attention_backend,
     new_flash_split_scratch,
     quantize_kv_fp8,

@@ -12,6 +12,7 @@ LIB_PATH = Path(__file__).resolve().parent / "lib" / "libruntherder_attn.so"
 
 _c_int = ctypes.c_int
 _vp = ctypes.c_void_p
+_i64 = ctypes.c_int64
 
 # name -> (restype, argtypes)
 _SIGNATURES = {
@@ -71,6 +72,21 @@ _SIGNATURES = {
     "rth_attn_prefill_split_paged": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _vp,
                                               _c_int, _c_int, _vp, _c_int, _c_int, _c_int,
                                               ctypes.c_float, _vp]),
+    "rth_attn_packed": (_c_int, [_vp] * 5 + [_c_int] * 2 + [_i64] * 4 + [_c_int] * 3 +
+                        [ctypes.c_float, _vp]),
+    "rth_kv_append_fp8_batch": (_c_int, [_vp] * 6 + [_i64] * 2 + [_vp] * 2 + [_c_int] * 4 +
+                                [_vp] + [_c_int] * 3 + [_vp]),
+    "rth_batch_scratch_floats": (ctypes.c_size_t, [_c_int] * 4),
+    "rth_attn_decode_batch": (_c_int, [_vp, _i64, _vp, _i64] + [_vp] * 5 + [_c_int] * 3 +
+                              [_vp, _vp, _c_int, _vp, _vp] + [_c_int] * 4 +
+                              [ctypes.c_float, _vp]),
+    "rth_pages_work_ints": (ctypes.c_size_t, [_c_int]),
+    "rth_pages_copy": (_c_int, [_vp] * 4 + [_c_int] * 5 + [_vp] * 2 + [_c_int, _vp]),
+    "rth_pages_reserve": (_c_int, [_vp] * 3 + [_c_int] * 2 + [_vp, _c_int, _vp, _vp, _c_int, _vp]),
+    "rth_pages_fork": (_c_int, [_vp] * 4 + [_c_int] * 5 + [_vp] * 7 + [_c_int] * 2 +
+                       [_vp, _c_int, _vp]),
+    "rth_pages_free": (_c_int, [_vp, _c_int, _vp, _c_int, _vp, _vp, _c_int, _vp]),
+    "rth_pages_compact": (_c_int, [_vp] * 4 + [_c_int] * 5 + [_vp] * 3 + [_c_int] * 2 + [_vp]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -43,6 +43,10 @@ KERNEL_SOURCES = [
     "attention_naive.hip",
     "rope.hip",
     "rmsnorm.hip",
+    "flash_packed.hip",
+    "flash_batch.hip",
+    "kv_batch.hip",
+    "pages.hip",
     "capi.cpp",
 ]
 HOST_SOURCES = ["attention_backends.cpp"]

@@ -198,6 +198,59 @@ int prefill_split_common(uint16_t* out, const uint16_t* q, const uint8_t* k, con
                                                      as_stream(stream), block_table, shift),
                      what);
 }
+constexpr int kMaxBatchSeqs = 4096;   // of one batch call (batch_common.hpp)
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int check_batch(int num_seqs) {
+    RTH_REQUIRE(num_seqs >= 1 && num_seqs <= kMaxBatchSeqs,
+                "num_seqs must be in [1, " + std::to_string(kMaxBatchSeqs) + "]");
+    return RTH_OK;
+}
+
+int check_row_stride(int64_t stride, int64_t heads, int head_dim, const char* name) {
+    RTH_REQUIRE(stride >= heads * head_dim && stride % 8 == 0,
+                std::string(name) + " must be a multiple of 8 and at least heads * head_dim");
+    return RTH_OK;
+}
+
+int check_tables(const void* tables, int table_blocks, int num_blocks, int block_size) {
+    RTH_REQUIRE(tables != nullptr, "block_tables must not be null");
+    RTH_REQUIRE(table_blocks >= 1, "table_blocks must be >= 1");
+    RTH_REQUIRE(num_blocks >= 1, "num_blocks must be >= 1");
+    RTH_REQUIRE(block_shift_of(block_size) >= 0, "block_size must be a power of two >= 32");
+    // Positions are 32-bit ints.
+    RTH_REQUIRE(static_cast<int64_t>(num_blocks) * block_size <= INT32_MAX,
+                "num_blocks * block_size must be below 2^31");
+    return RTH_OK;
+}
+
+int check_slabs(const void* k, const void* v, const void* ks, const void* vs) {
+    RTH_REQUIRE(k != nullptr && v != nullptr && ks != nullptr && vs != nullptr,
+                "k, v, k_scale and v_scale must not be null");
+    RTH_REQUIRE(aligned16(k) && aligned16(v), "k and v must be 16-byte aligned");
+    return RTH_OK;
+}
+
+int check_pool(const int* refs, int num_blocks, const int* tables, int table_blocks, int num_seqs) {
+    RTH_REQUIRE(refs != nullptr, "refs must not be null");
+    RTH_REQUIRE(num_blocks >= 1, "num_blocks must be >= 1");
+    RTH_REQUIRE(tables != nullptr, "block_tables must not be null");
+    RTH_REQUIRE(table_blocks >= 1, "table_blocks must be >= 1");
+    return check_batch(num_seqs);
+}
+
+int check_page_slabs(const rth::PageSlabs& s) {
+    if (int rc = check_slabs(s.k, s.v, s.ks, s.vs)) {
+        return rc;
+    }
+    RTH_REQUIRE(s.layers >= 1, "num_layers must be >= 1");
+    RTH_REQUIRE(s.num_blocks >= 1, "num_blocks must be >= 1");
+    RTH_REQUIRE(block_shift_of(s.block_size) >= 0, "block_size must be a power of two >= 32");
+    RTH_REQUIRE(s.hkv >= 1, "num_kv_heads must be >= 1");
+    RTH_REQUIRE(s.head_dim >= 8 && s.head_dim % 8 == 0, "head_dim must be a multiple of 8");
+    return RTH_OK;
+}
 }  // namespace
 
 extern "C" {
@@ -739,6 +792,224 @@ int rth_rmsnorm_bf16(uint16_t* y, const uint16_t* x, const uint16_t* g, int num_
 
 int rth_rmsnorm_lanes(int hidden_dim) {
     return (hidden_dim >= 8 && hidden_dim % 8 == 0) ? rth::rmsnorm_lanes(hidden_dim) : 0;
+}
+
+int rth_attn_packed(uint16_t* out, const uint16_t* q, const uint16_t* k, const uint16_t* v,
+                    const int* cu_seqlens, int num_seqs, int num_rows, int64_t out_stride,
+                    int64_t q_stride, int64_t k_stride, int64_t v_stride, int num_q_heads,
+                    int num_kv_heads, int head_dim, float scale, void* stream) {
+    RTH_REQUIRE(out != nullptr && q != nullptr && k != nullptr && v != nullptr,
+                "out, q, k and v must not be null");
+    RTH_REQUIRE(aligned16(out) && aligned16(q) && aligned16(k) && aligned16(v),
+                "out, q, k and v must be 16-byte aligned");
+    RTH_REQUIRE(cu_seqlens != nullptr, "cu_seqlens must not be null");
+    if (int rc = check_batch(num_seqs)) {
+        return rc;
+    }
+    if (int rc = check_heads(num_q_heads, num_kv_heads)) {
+        return rc;
+    }
+    RTH_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256,
+                "rth_attn_packed: head_dim must be one of 64, 128, 256");
+    RTH_REQUIRE(num_rows >= 1, "num_rows must be >= 1");
+    RTH_REQUIRE(static_cast<int64_t>(num_rows) * num_q_heads <= INT32_MAX,
+                "num_rows * num_q_heads must be below 2^31");
+    if (int rc = check_row_stride(out_stride, num_q_heads, head_dim, "out_stride")) {
+        return rc;
+    }
+    if (int rc = check_row_stride(q_stride, num_q_heads, head_dim, "q_stride")) {
+        return rc;
+    }
+    if (int rc = check_row_stride(k_stride, num_kv_heads, head_dim, "k_stride")) {
+        return rc;
+    }
+    if (int rc = check_row_stride(v_stride, num_kv_heads, head_dim, "v_stride")) {
+        return rc;
+    }
+    return check_hip(rth::flash_packed_launch(out, q, k, v, cu_seqlens, num_seqs, num_rows,
+                                              out_stride, q_stride, k_stride, v_stride, num_q_heads,
+                                              num_kv_heads, head_dim, scale, as_stream(stream)),
+                     "rth_attn_packed");
+}
+
+int rth_kv_append_fp8_batch(uint8_t* k_cache, uint8_t* v_cache, float* k_scale, float* v_scale,
+                            const uint16_t* k, const uint16_t* v, int64_t k_stride,
+                            int64_t v_stride, const int* cu_seqlens, const int* at_pos,
+                            int num_seqs, int num_rows, int num_kv_heads, int head_dim,
+                            const int* block_tables, int table_blocks, int num_blocks,
+                            int block_size, void* stream) {
+    if (int rc = check_slabs(k_cache, v_cache, k_scale, v_scale)) {
+        return rc;
+    }
+    RTH_REQUIRE(k != nullptr && v != nullptr, "k and v must not be null");
+    RTH_REQUIRE(aligned16(k) && aligned16(v), "k and v must be 16-byte aligned");
+    RTH_REQUIRE(at_pos != nullptr, "at_pos must not be null");
+    if (int rc = check_batch(num_seqs)) {
+        return rc;
+    }
+    RTH_REQUIRE(num_rows >= 1, "num_rows must be >= 1");
+    RTH_REQUIRE(num_kv_heads >= 1, "num_kv_heads must be >= 1");
+    RTH_REQUIRE(head_dim >= 8 && head_dim % 8 == 0 && head_dim <= 512,
+                "head_dim must be a multiple of 8 in [8, 512]");
+    RTH_REQUIRE(static_cast<int64_t>(num_rows) * num_kv_heads <= INT32_MAX,
+                "num_rows * num_kv_heads must be below 2^31");
+    if (int rc = check_row_stride(k_stride, num_kv_heads, head_dim, "k_stride")) {
+        return rc;
+    }
+    if (int rc = check_row_stride(v_stride, num_kv_heads, head_dim, "v_stride")) {
+        return rc;
+    }
+    if (int rc = check_tables(block_tables, table_blocks, num_blocks, block_size)) {
+        return rc;
+    }
+    return check_hip(rth::kv_append_batch_launch(k_cache, v_cache, k_scale, v_scale, k, v, k_stride,
+                                                 v_stride, cu_seqlens, at_pos, num_seqs, num_rows,
+                                                 num_kv_heads, head_dim, block_tables, table_blocks,
+                                                 num_blocks, block_shift_of(block_size),
+                                                 as_stream(stream)),
+                     "rth_kv_append_fp8_batch");
+}
+
+size_t rth_batch_scratch_floats(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim) {
+    int cus = 0;
+    if (num_seqs < 1 || num_seqs > kMaxBatchSeqs || num_q_heads < 1 || num_kv_heads < 1 ||
+        num_q_heads % num_kv_heads != 0 || head_dim < 1) {
+        return 0;
+    }
+    if (rth::device_cu_count(&cus) != hipSuccess) {
+        cus = 256;
+    }
+    return rth::batch_scratch_floats(num_seqs, num_q_heads, num_kv_heads, head_dim, cus);
+}
+
+int rth_attn_decode_batch(uint16_t* out, int64_t out_stride, const uint16_t* q, int64_t q_stride,
+                          const uint8_t* k, const uint8_t* v, const float* k_scale,
+                          const float* v_scale, const int* block_tables, int table_blocks,
+                          int num_blocks, int block_size, const int* lens,
+                          const int* prefix_table, int prefix_blocks, const int* prefix_len,
+                          float* partial, int num_seqs, int num_q_heads, int num_kv_heads,
+                          int head_dim, float scale, void* stream) {
+    RTH_REQUIRE(out != nullptr && q != nullptr, "out and q must not be null");
+    RTH_REQUIRE(aligned16(out) && aligned16(q), "out and q must be 16-byte aligned");
+    if (int rc = check_slabs(k, v, k_scale, v_scale)) {
+        return rc;
+    }
+    RTH_REQUIRE(lens != nullptr, "lens must not be null");
+    RTH_REQUIRE((prefix_table != nullptr) == (prefix_len != nullptr),
+                "prefix_table and prefix_len go together");
+    RTH_REQUIRE(prefix_table == nullptr || prefix_blocks >= 1, "prefix_blocks must be >= 1");
+    RTH_REQUIRE(partial != nullptr && aligned16(partial), "partial must be a 16-byte aligned buffer");
+    if (int rc = check_batch(num_seqs)) {
+        return rc;
+    }
+    if (int rc = check_heads(num_q_heads, num_kv_heads)) {
+        return rc;
+    }
+    RTH_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256,
+                "rth_attn_decode_batch: head_dim must be one of 64, 128, 256");
+    RTH_REQUIRE(static_cast<int64_t>(num_seqs) * num_q_heads <= (1 << 24),
+                "num_seqs * num_q_heads must be at most 2^24");
+    if (int rc = check_row_stride(out_stride, num_q_heads, head_dim, "out_stride")) {
+        return rc;
+    }
+    if (int rc = check_row_stride(q_stride, num_q_heads, head_dim, "q_stride")) {
+        return rc;
+    }
+    if (int rc = check_tables(block_tables, table_blocks, num_blocks, block_size)) {
+        return rc;
+    }
+    return check_hip(rth::flash_batch_launch(out, out_stride, q, q_stride, k, v, k_scale, v_scale,
+                                             block_tables, table_blocks, num_blocks,
+                                             block_shift_of(block_size), lens, prefix_table,
+                                             prefix_blocks, prefix_len, partial, num_seqs,
+                                             num_q_heads, num_kv_heads, head_dim, scale,
+                                             as_stream(stream)),
+                     "rth_attn_decode_batch");
+}
+
+size_t rth_pages_work_ints(int num_blocks) {
+    // Pages found (or new names), then a count and up to three lists.
+    return num_blocks < 1 ? 0 : 4 * static_cast<size_t>(num_blocks) + 4;
+}
+
+int rth_pages_copy(uint8_t* k, uint8_t* v, float* k_scale, float* v_scale, int num_layers,
+                   int num_blocks, int block_size, int num_kv_heads, int head_dim,
+                   const int* src, const int* dst, int count, void* stream) {
+    const rth::PageSlabs s{k, v, k_scale, v_scale, num_layers, num_blocks, block_size, num_kv_heads, head_dim};
+    if (int rc = check_page_slabs(s)) {
+        return rc;
+    }
+    RTH_REQUIRE(src != nullptr && dst != nullptr, "src and dst must not be null");
+    RTH_REQUIRE(count >= 1, "count must be >= 1");
+    return check_hip(rth::pages_copy_launch(s, src, dst, count, as_stream(stream)), "rth_pages_copy");
+}
+
+int rth_pages_reserve(int* refs, int* work, int* status, int num_blocks, int block_size,
+                      int* block_tables, int table_blocks, const int* lens, const int* n_new,
+                      int num_seqs, void* stream) {
+    if (int rc = check_pool(refs, num_blocks, block_tables, table_blocks, num_seqs)) {
+        return rc;
+    }
+    RTH_REQUIRE(work != nullptr && status != nullptr, "work and status must not be null");
+    RTH_REQUIRE(block_shift_of(block_size) >= 0, "block_size must be a power of two >= 32");
+    RTH_REQUIRE(lens != nullptr && n_new != nullptr, "lens and n_new must not be null");
+    return check_hip(rth::pages_reserve_launch(refs, work, status, num_blocks, block_size,
+                                               block_tables, table_blocks, lens, n_new, num_seqs,
+                                               as_stream(stream)),
+                     "rth_pages_reserve");
+}
+
+int rth_pages_fork(uint8_t* k, uint8_t* v, float* k_scale, float* v_scale, int num_layers,
+                   int num_blocks, int block_size, int num_kv_heads, int head_dim, int* refs,
+                   int* work, int* status, int* dst_tables, int* dst_lens,
+                   const int* src_tables, const int* src_lens, int table_blocks, int num_src,
+                   const int* parents, int num_children, void* stream) {
+    const rth::PageSlabs s{k, v, k_scale, v_scale, num_layers, num_blocks, block_size, num_kv_heads, head_dim};
+    if (int rc = check_page_slabs(s)) {
+        return rc;
+    }
+    if (int rc = check_pool(refs, num_blocks, src_tables, table_blocks, num_src)) {
+        return rc;
+    }
+    RTH_REQUIRE(work != nullptr && status != nullptr, "work and status must not be null");
+    RTH_REQUIRE(dst_tables != nullptr && dst_lens != nullptr && src_lens != nullptr && parents != nullptr,
+                "dst_tables, dst_lens, src_lens and parents must not be null");
+    RTH_REQUIRE(dst_tables != src_tables && dst_lens != src_lens,
+                "a fork writes tables and lengths of its own");
+    RTH_REQUIRE(num_children >= 1 && num_children <= kMaxBatchSeqs && num_children <= num_blocks,
+                "num_children must be in [1, min(4096, num_blocks)]");
+    return check_hip(rth::pages_fork_launch(s, refs, work, status, dst_tables, dst_lens, src_tables,
+                                            src_lens, table_blocks, num_src, parents, num_children,
+                                            as_stream(stream)),
+                     "rth_pages_fork");
+}
+
+int rth_pages_free(int* refs, int num_blocks, int* block_tables, int table_blocks, int* lens,
+                   const int* drop, int num_seqs, void* stream) {
+    if (int rc = check_pool(refs, num_blocks, block_tables, table_blocks, num_seqs)) {
+        return rc;
+    }
+    RTH_REQUIRE(lens != nullptr, "lens must not be null");
+    return check_hip(rth::pages_free_launch(refs, num_blocks, block_tables, table_blocks, lens, drop,
+                                            num_seqs, as_stream(stream)),
+                     "rth_pages_free");
+}
+
+int rth_pages_compact(uint8_t* k, uint8_t* v, float* k_scale, float* v_scale, int num_layers,
+                      int num_blocks, int block_size, int num_kv_heads, int head_dim, int* refs,
+                      int* work, int* block_tables, int table_blocks, int num_seqs,
+                      void* stream) {
+    const rth::PageSlabs s{k, v, k_scale, v_scale, num_layers, num_blocks, block_size, num_kv_heads, head_dim};
+    if (int rc = check_page_slabs(s)) {
+        return rc;
+    }
+    if (int rc = check_pool(refs, num_blocks, block_tables, table_blocks, num_seqs)) {
+        return rc;
+    }
+    RTH_REQUIRE(work != nullptr, "work must not be null");
+    return check_hip(rth::pages_compact_launch(s, refs, work, block_tables, table_blocks, num_seqs,
+                                               as_stream(stream)),
+                     "rth_pages_compact");
 }
 
 int rth_advance_position(int* pos, int delta, void* stream) {

@@ -135,4 +135,53 @@ int rmsnorm_lanes(int dim);
 hipError_t rmsnorm_bf16_launch(uint16_t* y, const uint16_t* x, const uint16_t* g, int rows,
                                int dim, float eps, hipStream_t stream);
 
+// Causal attention over packed prompts: sequence b holds rows cu_seqlens[b] ..
+// cu_seqlens[b + 1] - 1 of q, k, v and out (strides in elements per row).
+hipError_t flash_packed_launch(uint16_t* out, const uint16_t* q, const uint16_t* k,
+                               const uint16_t* v, const int* cu_seqlens, int num_seqs,
+                               int num_rows, int64_t out_stride, int64_t q_stride,
+                               int64_t k_stride, int64_t v_stride, int num_q_heads,
+                               int num_kv_heads, int head_dim, float scale, hipStream_t stream);
+
+// One token of each sequence over its pages, the first *prefix_len keys over
+// those of prefix_table (prefix_len may be null: none).
+std::size_t batch_scratch_floats(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
+                                 int cus);
+hipError_t flash_batch_launch(uint16_t* out, int64_t out_stride, const uint16_t* q,
+                              int64_t q_stride, const uint8_t* k, const uint8_t* v,
+                              const float* k_scale, const float* v_scale, const int* block_tables,
+                              int table_blocks, int num_blocks, int block_shift, const int* lens,
+                              const int* prefix_table, int prefix_blocks, const int* prefix_len,
+                              float* partial, int num_seqs, int num_q_heads, int num_kv_heads,
+                              int head_dim, float scale, hipStream_t stream);
+
+// The rows of a packed batch (cu_seqlens null: one row per sequence) into the
+// pages of their sequences, from position at_pos[b] on.
+hipError_t kv_append_batch_launch(uint8_t* k_q, uint8_t* v_q, float* k_scale, float* v_scale,
+                                  const uint16_t* k, const uint16_t* v, int64_t k_stride,
+                                  int64_t v_stride, const int* cu_seqlens, const int* at_pos,
+                                  int num_seqs, int num_rows, int num_kv_heads, int head_dim,
+                                  const int* block_tables, int table_blocks, int num_blocks,
+                                  int block_shift, hipStream_t stream);
+
+// The slabs of a paged cache over all its layers.
+struct PageSlabs {
+    uint8_t *k, *v;
+    float *  ks, *vs;
+    int      layers, num_blocks, block_size, hkv, head_dim;
+};
+hipError_t pages_copy_launch(const PageSlabs& s, const int* src, const int* dst, int count,
+                             hipStream_t stream);
+hipError_t pages_reserve_launch(int* refs, int* work, int* status, int num_blocks, int block_size,
+                                int* tables, int table_blocks, const int* lens, const int* n_new,
+                                int num_seqs, hipStream_t stream);
+hipError_t pages_fork_launch(const PageSlabs& s, int* refs, int* work, int* status,
+                             int* dst_tables, int* dst_lens, const int* src_tables,
+                             const int* src_lens, int table_blocks, int num_src,
+                             const int* parents, int num_children, hipStream_t stream);
+hipError_t pages_free_launch(int* refs, int num_blocks, int* tables, int table_blocks, int* lens,
+                             const int* drop, int num_seqs, hipStream_t stream);
+hipError_t pages_compact_launch(const PageSlabs& s, int* refs, int* work, int* tables,
+                                int table_blocks, int num_seqs, hipStream_t stream);
+
 }  // namespace rth

@@ -284,6 +284,129 @@ def rmsnorm_lanes(hidden_dim: int) -> int:
     return int(_ffi.load().rth_rmsnorm_lanes(hidden_dim))
 
 
+# ---- batches ---------------------------------------------------------------
+# No reference counterparts: the reference serves one sequence at a time.
+
+def _need_rows(t: torch.Tensor, heads: int, head_dim: int, name: str) -> int:
+    """t: [rows, heads, head_dim] bf16, rows any stride apart; the stride."""
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name} must be torch.bfloat16, got {t.dtype}")
+    if not t.is_cuda:
+        raise TypeError(f"{name} must be a device tensor")
+    if t.shape[1:] != (heads, head_dim):
+        raise ValueError(f"{name} must be [rows, {heads}, {head_dim}], got {tuple(t.shape)}")
+    s = t.stride()
+    if s[2] != 1 or s[1] != head_dim:
+        raise TypeError(f"{name}: a row's heads must be contiguous")
+    return s[0] if t.shape[0] > 1 else max(s[0], heads * head_dim)
+
+
+def _need_len(t: torch.Tensor, n: int, name: str) -> None:
+    _need(t, torch.int32, name)
+    if t.numel() != n:
+        raise ValueError(f"{name} must hold {n} ints, got {t.numel()}")
+
+
+def _need_tables(t: torch.Tensor, num_seqs: int, name: str = "block_tables") -> int:
+    """t: [num_seqs, table_blocks] int32; table_blocks."""
+    _need(t, torch.int32, name)
+    if t.dim() != 2 or t.shape[0] != num_seqs:
+        raise ValueError(f"{name} must be [{num_seqs}, blocks], got {tuple(t.shape)}")
+    return t.shape[1]
+
+
+def _need_slabs_of(k, v, k_scale, v_scale, block_size, num_kv_heads, head_dim) -> int:
+    """One layer's paged slabs; the number of blocks."""
+    _need(k, torch.uint8, "k"); _need(v, torch.uint8, "v")
+    _need(k_scale, torch.float32, "k_scale"); _need(v_scale, torch.float32, "v_scale")
+    rows = k.numel() // (num_kv_heads * head_dim)
+    if (block_size < 1 or rows % block_size or k.numel() != rows * num_kv_heads * head_dim
+            or v.numel() != k.numel() or k_scale.numel() != rows * num_kv_heads
+            or v_scale.numel() != k_scale.numel()):
+        raise ValueError("slabs must hold whole blocks of [block_size, kv heads, head_dim] codes "
+                         "and [block_size, kv heads] scales")
+    return rows // block_size
+
+
+def flash_packed_bf16(out, q, k, v, cu_seqlens, num_q_heads, num_kv_heads, head_dim, scale,
+                      stream=None):
+    """Causal attention over whole prompts packed one behind the other: rows
+    cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of q, out [rows, Hq, D] and k, v
+    [rows, Hkv, D] are sequence b. Rows may lie any stride apart (slices of a
+    fused projection); rows behind the last sequence stay as they are."""
+    so = _need_rows(out, num_q_heads, head_dim, "out")
+    sq = _need_rows(q, num_q_heads, head_dim, "q")
+    sk = _need_rows(k, num_kv_heads, head_dim, "k")
+    sv = _need_rows(v, num_kv_heads, head_dim, "v")
+    _need(cu_seqlens, torch.int32, "cu_seqlens")
+    n = q.shape[0]
+    if not (out.shape[0] == k.shape[0] == v.shape[0] == n):
+        raise ValueError("out, q, k and v must have the same number of rows")
+    _ffi.call("rth_attn_packed", _p(out), _p(q), _p(k), _p(v), _p(cu_seqlens),
+              cu_seqlens.numel() - 1, n, so, sq, sk, sv, num_q_heads, num_kv_heads, head_dim,
+              float(scale), _stream(stream))
+
+
+def kv_append_fp8_batch(k_cache, v_cache, k_scale, v_scale, k, v, at_pos, block_tables,
+                        block_size, num_kv_heads, head_dim, cu_seqlens=None, stream=None):
+    """Appends a batch's rows (k, v [rows, Hkv, D], packed by cu_seqlens, or
+    one row per sequence) to the pages of their sequences, sequence b from
+    position at_pos[b] on; bytes as PagedKVCache.append's. Rows without a page
+    are not stored."""
+    sk = _need_rows(k, num_kv_heads, head_dim, "k")
+    sv = _need_rows(v, num_kv_heads, head_dim, "v")
+    if k.shape[0] != v.shape[0]:
+        raise ValueError("k and v must have the same number of rows")
+    seqs = at_pos.numel()
+    _need(at_pos, torch.int32, "at_pos")
+    if cu_seqlens is not None:
+        _need_len(cu_seqlens, seqs + 1, "cu_seqlens")
+    elif k.shape[0] != seqs:
+        raise ValueError("without cu_seqlens, k and v hold one row per sequence")
+    width = _need_tables(block_tables, seqs)
+    blocks = _need_slabs_of(k_cache, v_cache, k_scale, v_scale, block_size, num_kv_heads, head_dim)
+    _ffi.call("rth_kv_append_fp8_batch", _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale), _p(k),
+              _p(v), sk, sv, _p(cu_seqlens), _p(at_pos), seqs, k.shape[0], num_kv_heads, head_dim,
+              _p(block_tables), width, blocks, block_size, _stream(stream))
+
+
+def batch_scratch_floats(num_seqs: int, num_q_heads: int, num_kv_heads: int,
+                         head_dim: int) -> int:
+    """Floats of flash_decode_batch_bf16's scratch on the current device."""
+    return int(_ffi.load().rth_batch_scratch_floats(num_seqs, num_q_heads, num_kv_heads, head_dim))
+
+
+def flash_decode_batch_bf16(out, q, k, v, k_scale, v_scale, block_tables, block_size, lens,
+                            partial, num_q_heads, num_kv_heads, head_dim, scale,
+                            prefix_table=None, prefix_len=None, stream=None):
+    """One query token of each sequence (q, out [seqs, Hq, D]) over keys
+    0 .. lens[b] - 1 of its pages. The first prefix_len[0] keys are shared: they
+    lie in the pages of prefix_table and are read once for the whole batch; the
+    others in block_tables[b], at their own positions. lens[b] <= 0: an unused
+    slot, zeros. partial: batch_scratch_floats floats."""
+    so = _need_rows(out, num_q_heads, head_dim, "out")
+    sq = _need_rows(q, num_q_heads, head_dim, "q")
+    seqs = q.shape[0]
+    if out.shape[0] != seqs:
+        raise ValueError("out and q must have the same number of rows")
+    _need_len(lens, seqs, "lens")
+    width = _need_tables(block_tables, seqs)
+    blocks = _need_slabs_of(k, v, k_scale, v_scale, block_size, num_kv_heads, head_dim)
+    _need(partial, torch.float32, "partial")
+    if partial.numel() < batch_scratch_floats(seqs, num_q_heads, num_kv_heads, head_dim):
+        raise ValueError("partial is smaller than batch_scratch_floats")
+    if (prefix_table is None) != (prefix_len is None):
+        raise ValueError("prefix_table and prefix_len go together")
+    if prefix_table is not None:
+        _need(prefix_table, torch.int32, "prefix_table")
+        _need_len(prefix_len, 1, "prefix_len")
+    _ffi.call("rth_attn_decode_batch", _p(out), so, _p(q), sq, _p(k), _p(v), _p(k_scale),
+              _p(v_scale), _p(block_tables), width, blocks, block_size, _p(lens),
+              _p(prefix_table), 0 if prefix_table is None else prefix_table.numel(),
+              _p(prefix_len), _p(partial), seqs, num_q_heads, num_kv_heads, head_dim,
+              float(scale), _stream(stream))
+
+
 # ---- interface -------------------------------------------------------------
 
 @dataclass(frozen=True)
@@ -321,6 +444,19 @@ class KVSlabs(KVView):
     def view(self) -> KVView:
         return KVView(self.k, self.v, self.k_scale, self.v_scale, self.block_table,
                       self.block_size)
+
+
+@dataclass(frozen=True)
+class KVBatchView:
+    """One layer of a paged cache with the block tables of a batch
+    (PagedKVCache.batch_view): block_tables [seqs, table_blocks] int32, entries
+    < 0 hold no page. No reference counterpart."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    block_tables: torch.Tensor
+    block_size: int
 
 
 def _need_slabs(kv):
@@ -435,6 +571,119 @@ class PagedKVCache:
         _need(block_table, torch.int32, "block_table")
         return KVSlabs(self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer],
                        block_table, self.block_size)
+
+    def append_batch(self, layer, k, v, at_pos, block_tables, cu_seqlens=None, stream=None):
+        """kv_append_fp8_batch into this layer: the rows of a packed batch
+        (cu_seqlens), or one row per sequence, at at_pos[b] of sequence b."""
+        if not 0 <= layer < self.num_layers:
+            raise ValueError("KVCache append layer out of range")
+        kv_append_fp8_batch(self.k[layer], self.v[layer], self.k_scale[layer],
+                            self.v_scale[layer], k, v, at_pos, block_tables, self.block_size,
+                            self.num_kv_heads, self.head_dim, cu_seqlens, stream)
+
+    def batch_view(self, layer, block_tables) -> KVBatchView:
+        if not 0 <= layer < self.num_layers:
+            raise ValueError("KVCache view layer out of range")
+        _need(block_tables, torch.int32, "block_tables")
+        if block_tables.dim() != 2:
+            raise ValueError("block_tables must be [seqs, blocks]")
+        return KVBatchView(self.k[layer], self.v[layer], self.k_scale[layer],
+                           self.v_scale[layer], block_tables, self.block_size)
+
+    def _all(self):
+        return (_p(self.k), _p(self.v), _p(self.k_scale), _p(self.v_scale), self.num_layers,
+                self.num_blocks, self.block_size, self.num_kv_heads, self.head_dim)
+
+    def copy_pages(self, src, dst, stream=None):
+        """Copies page src[i] to page dst[i] in every layer. The dst pages are
+        distinct and none of them is a src page."""
+        _need(src, torch.int32, "src")
+        _need_len(dst, src.numel(), "dst")
+        if src.numel():
+            _ffi.call("rth_pages_copy", *self._all(), _p(src), _p(dst), src.numel(),
+                      _stream(stream))
+
+
+class PagePool:
+    """Which pages of a paged cache are in use, on the device: refs[page]
+    counts the block-table entries that hold it, refs <= 0 is free, and the
+    lowest free pages are given out first. Block tables are [seqs, blocks]
+    int32 with -1 where there is no page (new_tables). Nothing here waits for
+    the device: what a call could not do for lack of pages (or of table
+    entries) it leaves undone and says in `status`, which stays set until
+    the caller clears it. Calls on one pool run one behind the other. No
+    reference counterpart."""
+
+    OUT_OF_PAGES, TABLE_TOO_SHORT = 1, 2   # bits of status
+
+    def __init__(self, num_blocks, block_size, device="cuda"):
+        if num_blocks < 1:
+            raise ValueError("PagePool num_blocks must be >= 1")
+        if block_size < 32 or block_size & (block_size - 1):
+            raise ValueError("PagePool block_size must be a power of two >= 32")
+        self.num_blocks, self.block_size, self.device = num_blocks, block_size, device
+        self.refs = torch.zeros(num_blocks, dtype=torch.int32, device=device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)
+        self._work = torch.empty(int(_ffi.load().rth_pages_work_ints(num_blocks)),
+                                 dtype=torch.int32, device=device)
+
+    def new_tables(self, num_seqs, table_blocks):
+        """Block tables without pages."""
+        return torch.full((num_seqs, table_blocks), -1, dtype=torch.int32, device=self.device)
+
+    def _of(self, cache):
+        if cache.num_blocks != self.num_blocks or cache.block_size != self.block_size:
+            raise ValueError("the pool and the cache differ in their blocks")
+
+    def reserve(self, block_tables, lens, n_new, stream=None):
+        """Pages for positions lens[b] .. lens[b] + n_new[b] - 1 of sequence b,
+        where its table row has none yet."""
+        _need(lens, torch.int32, "lens")
+        seqs = lens.numel()
+        _need_len(n_new, seqs, "n_new")
+        width = _need_tables(block_tables, seqs)
+        _ffi.call("rth_pages_reserve", _p(self.refs), _p(self._work), _p(self.status),
+                  self.num_blocks, self.block_size, _p(block_tables), width, _p(lens), _p(n_new),
+                  seqs, _stream(stream))
+
+    def fork(self, cache, dst_tables, dst_lens, src_tables, src_lens, parents, stream=None):
+        """Sequence i of dst becomes a copy of sequence parents[i] of src (any
+        number of children of one parent; a parent outside src gives an empty
+        one): filled pages are shared, a part-filled last page is copied, in all
+        layers of `cache`, into a page of the child's own. The dst tables hold no
+        pages before (free them first)."""
+        self._of(cache)
+        _need(parents, torch.int32, "parents"); _need(src_lens, torch.int32, "src_lens")
+        n = parents.numel()
+        _need_len(dst_lens, n, "dst_lens")
+        width = _need_tables(src_tables, src_lens.numel(), "src_tables")
+        if _need_tables(dst_tables, n, "dst_tables") != width:
+            raise ValueError("dst_tables and src_tables must have the same number of blocks")
+        _ffi.call("rth_pages_fork", *cache._all(), _p(self.refs), _p(self._work), _p(self.status),
+                  _p(dst_tables), _p(dst_lens), _p(src_tables), _p(src_lens), width,
+                  src_lens.numel(), _p(parents), n, _stream(stream))
+
+    def free(self, block_tables, lens, drop=None, stream=None):
+        """Frees the sequences with drop[b] != 0 (None: all): their pages lose
+        one reference, their table rows hold none, their lengths are 0."""
+        _need(lens, torch.int32, "lens")
+        seqs = lens.numel()
+        width = _need_tables(block_tables, seqs)
+        if drop is not None:
+            _need_len(drop, seqs, "drop")
+        _ffi.call("rth_pages_free", _p(self.refs), self.num_blocks, _p(block_tables), width,
+                  _p(lens), _p(drop), seqs, _stream(stream))
+
+    def compact(self, cache, block_tables, stream=None):
+        """Moves the pages in use down to the lowest ones, in all layers of
+        `cache`, and renames them in block_tables, which are all the tables that
+        hold pages of the pool."""
+        self._of(cache)
+        if block_tables.dim() != 2:
+            raise ValueError("block_tables must be [seqs, blocks]")
+        width = _need_tables(block_tables, block_tables.shape[0])
+        _ffi.call("rth_pages_compact", *cache._all(), _p(self.refs), _p(self._work),
+                  _p(block_tables), width, block_tables.shape[0], _stream(stream))
 
 
 class AttentionBackend:
@@ -579,6 +828,40 @@ class AdaptiveAttention(AttentionBackend):
             out, q, kv.k, kv.v, kv.k_scale, kv.v_scale, k_new, v_new, q_norm, k_norm, eps,
             positions, inv_freq, self.partial, self.num_splits, cache_len, c.num_q_heads,
             c.num_kv_heads, c.head_dim, c.scale, stream)
+
+
+class BatchAttention:
+    """Attention of a batch of up to max_seqs sequences: whole prompts packed
+    one behind the other, and one token of each sequence over a paged cache
+    whose first pages all may share. Owns the decode's scratch, so calls of
+    one object run one behind the other (one stream, or ordered streams; a
+    captured graph counts). No reference counterpart."""
+
+    def __init__(self, config: AttnConfig, max_seqs: int, device="cuda"):
+        if max_seqs < 1:
+            raise ValueError("BatchAttention max_seqs must be >= 1")
+        self.config, self.max_seqs = config, max_seqs
+        with torch.cuda.device(device):
+            n = max(batch_scratch_floats(b, config.num_q_heads, config.num_kv_heads,
+                                         config.head_dim)
+                    for b in range(1, max_seqs + 1))
+            self.partial = torch.empty(n, dtype=torch.float32, device=device)
+
+    def run_packed(self, out, q, k, v, cu_seqlens, stream=None):
+        """flash_packed_bf16 with this configuration (max_seqs does not bind it)."""
+        c = self.config
+        flash_packed_bf16(out, q, k, v, cu_seqlens, c.num_q_heads, c.num_kv_heads, c.head_dim,
+                          c.scale, stream)
+
+    def run_decode(self, out, q, kv: KVBatchView, lens, prefix_table=None, prefix_len=None,
+                   stream=None):
+        """flash_decode_batch_bf16 over kv with this object's scratch."""
+        c = self.config
+        if q.shape[0] > self.max_seqs:
+            raise ValueError(f"{q.shape[0]} sequences: this backend was made for {self.max_seqs}")
+        flash_decode_batch_bf16(out, q, kv.k, kv.v, kv.k_scale, kv.v_scale, kv.block_tables,
+                                kv.block_size, lens, self.partial, c.num_q_heads, c.num_kv_heads,
+                                c.head_dim, c.scale, prefix_table, prefix_len, stream)
 
 
 class NaiveAttention(AttentionBackend):

@@ -1,0 +1,106 @@
+"""Causal attention over packed prompts (no reference counterpart) against the
+formula in 64 bits: lengths from none to several tiles and row blocks, head
+groups, strides, padding, what masked places may hold, refusals."""
+import math
+
+import pytest
+import torch
+
+import runtherder_amd as R
+from batch_util import assert_attention, attend64, cu_of, ints, normal, score_size
+from gpu_util import DEV, step, sync
+
+pytestmark = pytest.mark.gpu
+
+
+def run(q, k, v, cu, out=None, scale=None, stream=None):
+    hq, d = q.shape[1:]
+    out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device=DEV) if out is None else out
+    R.flash_packed_bf16(out, q, k, v, cu, hq, k.shape[1], d,
+                        d ** -0.5 if scale is None else scale, stream)
+    return out
+
+
+def check(lens, hq, hkv, d, seed, fused=False, pad=0, rows=None, scale=None, size=1.0):
+    n = sum(lens) + pad
+    if fused:
+        x = normal((n, hq + 2 * hkv, d), seed, size)
+        q, k, v = x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:]
+        xd = x.to(DEV)
+        qd, kd, vd = xd[:, :hq], xd[:, hq:hq + hkv], xd[:, hq + hkv:]
+    else:
+        q, k, v = normal((n, hq, d), seed, size), normal((n, hkv, d), seed + 1), normal((n, hkv, d), seed + 2)
+        qd, kd, vd = q.to(DEV), k.to(DEV), v.to(DEV)
+    step(f"packed lens={lens} hq={hq} hkv={hkv} d={d} fused={fused} pad={pad}")
+    scale = d ** -0.5 if scale is None else scale
+    out = run(qd, kd, vd, ints(cu_of(lens)), scale=scale)
+    sync()
+    got, cu = out.cpu(), cu_of(lens)
+    for b, m in enumerate(lens):
+        picked = range(m) if m <= 80 else sorted({0, 1, 31, 32, 63, 64, m - 1, m - 2, m // 2,
+                                                  *(rows or ()), *range(7, m, max(1, m // 40))})
+        for t in picked:
+            if t >= m:
+                continue
+            at = cu[b]
+            want, weight = attend64(q[at + t], k[at:at + t + 1], v[at:at + t + 1], scale)
+            assert_attention(got[at + t], want, weight,
+                             score_size(q[at + t], k[at:at + t + 1], scale))
+    assert (got[cu[-1]:] == 7.0).all()   # rows behind the last sequence stay as they were
+
+
+@pytest.mark.parametrize("lens", [
+    [1], [2], [33], [64], [65], [127, 1, 0, 128], [0, 0, 5], [1] * 70, [300, 0, 17, 513, 64, 1],
+])
+def test_lengths(lens):
+    check(lens, 8, 2, 128, 100 + len(lens) + lens[0])
+
+
+@pytest.mark.parametrize("hq,hkv,d", [
+    (4, 4, 64), (16, 2, 64), (7, 1, 64), (8, 8, 128), (24, 8, 128), (28, 4, 128), (40, 1, 128),
+    (5, 1, 128), (4, 2, 256), (16, 4, 256), (9, 3, 256),
+])
+def test_heads(hq, hkv, d):
+    check([130, 3, 77], hq, hkv, d, 200 + hq + d)
+
+
+@pytest.mark.parametrize("lens,hq,hkv,d", [
+    ([1500, 40], 32, 8, 128), ([2049], 16, 8, 64), ([1100, 900], 8, 4, 256), ([4100], 8, 8, 128),
+])
+def test_long(lens, hq, hkv, d):
+    check(lens, hq, hkv, d, 300 + lens[0], rows=[1023, 1024, 1025])
+
+
+def test_slices_of_a_projection_with_padding():
+    check([200, 31, 64], 32, 8, 128, 400, fused=True, pad=9)
+    check([70, 1], 6, 2, 256, 401, fused=True, pad=1)
+    check([90, 5], 6, 2, 64, 402, fused=True, pad=300)
+
+
+def test_score_ranges():
+    """Scores far apart: the reference maximum moves, or lies far above most keys."""
+    check([400, 90], 8, 2, 128, 500, size=30.0)
+    check([400], 8, 2, 64, 501, scale=8.0)
+    check([130], 4, 1, 256, 502, scale=0.0)
+    # Scores that grow along the keys, then fall.
+    n, d = 320, 128
+    ramp = torch.cat([torch.arange(160.0), torch.arange(160.0, 0, -1)])[:, None, None]
+    q = torch.full((n, 2, d), 1.0).to(torch.bfloat16)
+    k = (ramp / 4 + torch.zeros(n, 1, d)).to(torch.bfloat16)
+    v = normal((n, 1, d), 503)
+    out = run(q.to(DEV), k.to(DEV), v.to(DEV), ints([0, n])).cpu()
+    for t in range(0, n, 7):
+        want, weight = attend64(q[t], k[:t + 1], v[:t + 1], d ** -0.5)
+        assert_attention(out[t], want, weight, score_size(q[t], k[:t + 1], d ** -0.5))
+
+
+def test_repeats_bit_for_bit_and_on_a_stream():
+    q, k, v = (normal((700, h, 128), 600 + h).to(DEV) for h in (16, 4, 4))
+    cu = ints([0, 300, 301, 700])
+    a = run(q, k, v, cu)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    b = torch.empty_like(a)
+    run(q, k, v, cu, out=b, stream=s)
+    s.synchronize()
+    assert torch.equal(a, b)
