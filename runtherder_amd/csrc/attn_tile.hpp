@@ -1,5 +1,5 @@
-// The tile step of the batch attention kernels: query rows in registers against
-// a tile of keys whose K and V rows lie in LDS as bf16.
+// The tile loop of the batch attention kernels: query rows in registers against
+// tiles of keys whose K and V rows lie in LDS as bf16.
 #pragma once
 
 #include "batch_common.hpp"
@@ -9,176 +9,234 @@ namespace rth {
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kPW   = 4;    // waves per workgroup
-constexpr int kPThr = kPW * kWave;
-
 // Rows of a K or V tile in LDS: 16 bytes between K rows spread the operand
 // reads (16 bytes of 32 rows) over the banks, 64 bytes those of V^T (64 bytes
-// of four rows).
+// of four rows). K and V have two buffers each, tile i in buffer i % 2.
 template <int D>
 struct AttnTile {
-    static constexpr int kN      = D == 256 ? 32 : 64;   // keys
+    static constexpr int kN      = 64;   // keys
     static constexpr int kKPitch = 2 * D + 16;
     static constexpr int kVPitch = 2 * D + 64;
     static constexpr int kK      = kN * kKPitch;
-    static constexpr int kBytes  = kK + kN * kVPitch;
+    static constexpr int kV      = kN * kVPitch;
+    static constexpr int kBytes  = 2 * (kK + kV);
+    static __device__ __forceinline__ uint32_t k_at(int tile) { return (tile & 1) * kK; }
+    static __device__ __forceinline__ uint32_t v_at(int tile) { return 2 * kK + (tile & 1) * kV; }
 };
 
-// 32 kQ query rows of a wave (lane l: rows l % 32 of each block of 32) and what
-// they have gathered: S^T = K Q^T and O^T += V^T P^T on
-// v_mfma_f32_32x32x16_bf16, so that a lane owns a query row and the softmax
-// needs no lane exchange but for a new maximum; P^T goes from the score
-// registers into the second product as it is, because V^T is read
-// (ds_read_b64_tr_b16) in the scores' key order. Softmax in base 2, fp32, with a
-// lazy reference maximum: it moves at the first keys, and when a row's sum of 32
-// weights passes 2^20; one reference for the sum and for O, so the result
-// does not depend on it. P is rounded to bf16 (half a step, 2^-9 of each weight)
-// for the matrix product, the row sum takes the fp32 values.
-template <int D, int kQ>
-struct QueryRows {
-    static constexpr int kKS = D / 16;   // k-steps of a score
-    static constexpr int kDB = D / 32;   // d blocks of O^T
+// Keeps the instruction scheduler from moving anything across.
+__device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
 
-    bf16x8 qf[kQ][kKS];   // k-step s of lane (row, h): d = 16 s + 8 h .. + 7
-    f32x16 o[kQ][kDB];
-    float  m_ref[kQ], l_run[kQ];
-    bool   start;
+// 32 query rows of a wave (lane l: row l % 32) and what they have gathered.
+// S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16_bf16, so that a lane
+// owns a query row and the softmax needs no lane exchange but for a new maximum;
+// P^T goes from the score registers into the second product as it is, because
+// V^T is read (ds_read_b64_tr_b16) in the scores' key order. Softmax in base 2,
+// fp32, with a lazy reference maximum: it moves at the first keys, and when a
+// row's sum of 32 weights passes 2^20; one reference for the sum and for O, so
+// the result does not depend on it. P is rounded to bf16 (half a step, 2^-9 of
+// each weight) for the matrix product, the row sum takes the fp32 values.
+//
+// Software pipelined by halves of a tile (32 keys): one step does the softmax
+// of half j under the P V products of half j - 1 and the scores of half j + 1,
+// which alternate (neither waits for the other) in the order written here.
+// kPrio (one workgroup of two waves per SIMD): a wave holds priority over the
+// first two thirds of a step, so that it does not give up its place between
+// its MFMAs; held to the end, the other wave's came in too late.
+// kScaled: every key has a factor of its own for its scores (times scale *
+// log2 e) and one for its values, read from LDS; else all share scale_log2.
+template <int D, bool kScaled, bool kPrio>
+struct QueryRows {
+    using T = AttnTile<D>;
+    static constexpr int kSteps = D / 16;   // MFMAs of a half's scores, and of its P V
+    static constexpr int kDB    = D / 32;   // d blocks of O^T
+    static constexpr int kAhead = 3;        // operand reads ahead of their MFMA
+
+    bf16x8 qf[kSteps];   // k-step c of lane (row, h): d = 16 c + 8 h .. + 7
+    f32x16 o[kDB];
+    f32x16 s[2];         // scores of half j in s[j % 2]
+    bf16x8 p[2];         // P^T of the half before
+    bf16x8 ka[kAhead + 1], va[kAhead + 1];
+    float  m_ref, l_run;
+    int    lane;
 
     __device__ __forceinline__ void clear() {
-        start = true;
-#pragma unroll
-        for (int a = 0; a < kQ; ++a) {
-            m_ref[a] = 0.0f;
-            l_run[a] = 0.0f;
-#pragma unroll
-            for (int b = 0; b < kDB; ++b) {
-                o[a][b] = f32x16{};
-            }
-        }
-    }
-
-    __device__ __forceinline__ void load_q(int a, const uint16_t* row, int h) {
-#pragma unroll
-        for (int s = 0; s < kKS; ++s) {
-            qf[a][s] = *reinterpret_cast<const bf16x8*>(row + 16 * s + 8 * h);
-        }
-    }
-
-    // Keys 32 hf .. + 31 of the tile at kb, vb. kScaled: kf, vf hold the tile's
-    // key factors (times scale * log2 e) and value factors, else every key's
-    // factor is scale_log2. masked: key r of the half counts for block a as
-    // far as r <= lim[a] (lim: less 4 h).
-    template <bool kScaled>
-    __device__ __forceinline__ void half(const uint8_t* kb, const uint8_t* vb, int hf, int lane,
-                                         float scale_log2, const float* kf, const float* vf,
-                                         bool masked, const int (&lim)[kQ]) {
-        using T       = AttnTile<D>;
-        const int col = lane & 31, h = lane >> 5;
-        if constexpr (D == 256) {   // operand reads ahead of the marks would not fit the registers
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        f32x16    s[kQ];
-#pragma unroll
-        for (int a = 0; a < kQ; ++a) {
-            s[a] = f32x16{};
-        }
-#pragma unroll
-        for (int c = 0; c < kKS; ++c) {
-            const bf16x8 x = *reinterpret_cast<const bf16x8*>(kb + (32 * hf + col) * T::kKPitch +
-                                                              32 * c + 16 * h);
-#pragma unroll
-            for (int a = 0; a < kQ; ++a) {
-                s[a] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, qf[a][c], s[a], 0, 0, 0);
-            }
-            if constexpr (D == 256) {
-                if (c % 4 == 3) {
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            }
-        }
-        // Register e of a lane: key 8 (e / 4) + 4 h + e % 4 of the half.
-        f32x4 fk[4], fv[4];
-        if constexpr (kScaled) {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                fk[g] = *reinterpret_cast<const f32x4*>(kf + 32 * hf + 8 * g + 4 * h);
-                fv[g] = *reinterpret_cast<const f32x4*>(vf + 32 * hf + 8 * g + 4 * h);
-            }
-        }
-        bf16x8 p[kQ][2];
-        float  sum[kQ];
-        auto   weights = [&](int a) {
-            float t0 = 0.0f, t1 = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float x = __builtin_amdgcn_exp2f(s[a][e]);
-                ((e & 1) != 0 ? t1 : t0) += x;
-                p[a][e >> 3][e & 7] = static_cast<__bf16>(kScaled ? x * fv[e >> 2][e & 3] : x);
-            }
-            sum[a] = t0 + t1;
-        };
-#pragma unroll
-        for (int a = 0; a < kQ; ++a) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                s[a][e] = fmaf(s[a][e], kScaled ? fk[e >> 2][e & 3] : scale_log2, -m_ref[a]);
-            }
-            if (masked) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    s[a][e] = 8 * (e >> 2) + (e & 3) > lim[a] ? -INFINITY : s[a][e];
-                }
-            }
-            weights(a);
-            if (start || __any(!(sum[a] <= 0x1p20f))) {
-                float top = s[a][0];
-#pragma unroll
-                for (int e = 1; e < 16; ++e) {
-                    top = fmaxf(top, s[a][e]);
-                }
-                top = wave_xor_max(top, 32);
-                const float up    = start ? (top == -INFINITY ? 0.0f : top) : fmaxf(top, 0.0f);
-                const float alpha = start ? 1.0f : __builtin_amdgcn_exp2f(-up);
-                m_ref[a] += up;
-                l_run[a] *= alpha;
-#pragma unroll
-                for (int b = 0; b < kDB; ++b) {
-                    o[a][b] *= alpha;
-                }
-                s[a] -= up;
-                weights(a);
-            }
-            l_run[a] += sum[a];
-        }
-        start = false;
-        // V^T: lane (d, h), keys 16 c + 4 h .. + 3 and 16 c + 8 + 4 h .. + 3. A
-        // group of 16 lanes reads four keys' 16 d and gets them transposed: lane i
-        // points at four d of key i / 4.
-        const int l16 = lane & 15;
-        const uint8_t* vp = vb + (32 * hf + 4 * h + (l16 >> 2)) * T::kVPitch +
-                            32 * ((lane >> 4) & 1) + 8 * (l16 & 3);
+        m_ref = 0.0f;
+        l_run = 0.0f;
 #pragma unroll
         for (int b = 0; b < kDB; ++b) {
+            o[b] = f32x16{};
+        }
+        p[0] = bf16x8{};
+        p[1] = bf16x8{};
+    }
+
+    __device__ __forceinline__ void load_q(const uint16_t* row) {
+        const int h = lane >> 5;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                typedef __attribute__((address_space(3))) s16x4* LdsPtr;
-                const uint8_t* at = vp + 16 * c * T::kVPitch + 64 * b;
-                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (LdsPtr)const_cast<uint8_t*>(at));
-                const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (LdsPtr)const_cast<uint8_t*>(at + 8 * T::kVPitch));
-                const s16x8  xy = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-                const bf16x8 va = __builtin_bit_cast(bf16x8, xy);
+        for (int c = 0; c < kSteps; ++c) {
+            qf[c] = *reinterpret_cast<const bf16x8*>(row + 16 * c + 8 * h);
+        }
+    }
+
+    // K operand of k-step c of the half whose K rows start at `at`: lane
+    // (key, h), d = 16 c + 8 h .. + 7.
+    __device__ __forceinline__ void read_k(const uint8_t* at, int c) {
+        ka[c & kAhead] = *reinterpret_cast<const bf16x8*>(at + (lane & 31) * T::kKPitch + 32 * c +
+                                                          16 * (lane >> 5));
+    }
+    // V^T operand of MFMA c of a half's P V (d block c % kDB, 16 keys c / kDB):
+    // lane (d, h), keys 4 h .. + 3 and 8 + 4 h .. + 3 of them. A group of 16
+    // lanes reads four keys' 16 d and gets them transposed: lane i points at four
+    // d of key i / 4.
+    __device__ __forceinline__ void read_v(const uint8_t* at, int c) {
+        typedef __attribute__((address_space(3))) s16x4* LdsPtr;
+        const int      l16 = lane & 15;
+        const uint8_t* x   = at + (4 * (lane >> 5) + (l16 >> 2)) * T::kVPitch +
+                           32 * ((lane >> 4) & 1) + 8 * (l16 & 3) + 16 * (c / kDB) * T::kVPitch +
+                           64 * (c % kDB);
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)const_cast<uint8_t*>(x));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (LdsPtr)const_cast<uint8_t*>(x + 8 * T::kVPitch));
+        const s16x8 ab = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        va[c & kAhead] = __builtin_bit_cast(bf16x8, ab);
+    }
+    __device__ __forceinline__ void qk(f32x16& x, int c) {
+        x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[c & kAhead], qf[c], c == 0 ? f32x16{} : x, 0, 0, 0);
+    }
+    __device__ __forceinline__ void pv(int c) {
+        o[c % kDB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[c & kAhead], p[c / kDB], o[c % kDB], 0, 0, 0);
+    }
+
+    // The operand reads that a step starts with.
+    __device__ __forceinline__ void head(const uint8_t* k_at, const uint8_t* v_at) {
 #pragma unroll
-                for (int a = 0; a < kQ; ++a) {
-                    o[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, p[a][c], o[a][b], 0, 0, 0);
+        for (int c = 0; c < kAhead; ++c) {
+            read_k(k_at, c);
+            read_v(v_at, c);
+        }
+    }
+
+    // Scores of the first half, before the first step.
+    __device__ __forceinline__ void first_scores(const uint8_t* k_at) {
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c) {
+            read_k(k_at, c);
+            qk(s[0], c);
+        }
+    }
+
+    // Softmax of half j (in s[kPar], kPar = j % 2), P V of half j - 1 (V rows from v_at),
+    // scores of half j + 1 (K rows from k_at), after head(k_at, v_at).
+    // masked: key r of half j counts as far as r <= lim (lim: less 4 h). kf, vf: the
+    // factors of half j.
+    template <int kPar>
+    __device__ __forceinline__ void step(const uint8_t* k_at, const uint8_t* v_at, float scale_log2,
+                                         const float* kf, const float* vf, bool start, bool masked,
+                                         int lim) {
+        f32x16&   x = s[kPar];
+        f32x16&   y = s[kPar ^ 1];
+        const int h = lane >> 5;
+        f32x4     fv[4];
+        bf16x8    pn[2];
+        float     sum[2] = {0.0f, 0.0f};
+        // Register e of a lane: key 8 (e / 4) + 4 h + e % 4 of the half.
+        auto scale4 = [&](int g) {
+            f32x4 f = {scale_log2, scale_log2, scale_log2, scale_log2};
+            if constexpr (kScaled) {
+                f     = *reinterpret_cast<const f32x4*>(kf + 8 * g + 4 * h);
+                fv[g] = *reinterpret_cast<const f32x4*>(vf + 8 * g + 4 * h);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[4 * g + e] = fmaf(x[4 * g + e], f[e], -m_ref);
+            }
+        };
+        auto exp4 = [&](int g) {
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                w[e] = __builtin_amdgcn_exp2f(x[4 * g + e]);
+                sum[e & 1] += w[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                pn[g >> 1][4 * (g & 1) + e] = static_cast<__bf16>(kScaled ? w[e] * fv[g][e] : w[e]);
+            }
+        };
+        scale4(0);
+        scale4(1);
+        pin();
+        if constexpr (kPrio) {
+            __builtin_amdgcn_s_setprio(1);
+        }
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c) {
+            pv(c);
+            if (c + kAhead < kSteps) {
+                read_v(v_at, c + kAhead);
+            }
+            if (c == 0) {
+                scale4(2);
+                scale4(3);
+            }
+            pin();
+            if (c == 0 && masked) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    x[e] = 8 * (e >> 2) + (e & 3) > lim ? -INFINITY : x[e];
                 }
             }
-            if constexpr (D == 256) {
-                if (b % 2 == 1) {
-                    __builtin_amdgcn_sched_barrier(0);
+            qk(y, c);
+            if (c + kAhead < kSteps) {
+                read_k(k_at, c + kAhead);
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                if (c == 1 + g * (kSteps - 1) / 4 || (kSteps == 4 && c == 3 && 1 + g * 3 / 4 > 3)) {
+                    exp4(g);
                 }
             }
+            pin();
+            if constexpr (kPrio) {
+                if (c == 2 * kSteps / 3) {
+                    __builtin_amdgcn_s_setprio(0);
+                }
+            }
+        }
+        if (__any(start || !(sum[0] + sum[1] <= 0x1p20f))) {
+            float top = x[0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) {
+                top = fmaxf(top, x[e]);
+            }
+            top               = wave_xor_max(top, 32);
+            const float up    = start ? (top == -INFINITY ? 0.0f : top) : fmaxf(top, 0.0f);
+            const float alpha = start ? 1.0f : __builtin_amdgcn_exp2f(-up);
+            m_ref += up;
+            l_run *= alpha;
+#pragma unroll
+            for (int b = 0; b < kDB; ++b) {
+                o[b] *= alpha;
+            }
+            x -= up;
+            sum[0] = sum[1] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                exp4(g);
+            }
+        }
+        l_run += sum[0] + sum[1];
+        p[0] = pn[0];
+        p[1] = pn[1];
+    }
+
+    // P V of the last half.
+    __device__ __forceinline__ void last(const uint8_t* v_at) {
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c) {
+            read_v(v_at, c);
+            pv(c);
         }
     }
 };

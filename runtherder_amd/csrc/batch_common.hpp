@@ -20,6 +20,10 @@ __device__ __forceinline__ int again(int x) {
     return x;
 }
 
+// x, the same in every lane, in a scalar register (a division leaves it in
+// vector ones).
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // Sum over the wave, in every lane: lane exchanges within rows of 16, then the
 // two cross-row swaps. Every lane must be active.
 __device__ __forceinline__ int wave_sum_i(int v) {

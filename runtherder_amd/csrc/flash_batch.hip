@@ -2,33 +2,40 @@
 // OCP E4M3 cache, the sequences sharing the pages of a prefix, gfx950.
 //
 // For sequence b and q head h of kv head h / G: out[b, h] = sum over keys
-// p < lens[b] of softmax_p(scale * scale * q[b, h] . k[p, h / G]) v[p, h / G]; the
-// first prefix_len keys lie in the pages of the prefix table for every
-// sequence, the others in the sequence's own table. lens[b] <= 0: zeros.
+// p < lens[b] of softmax_p(scale * q[b, h] . k[p, h / G]) v[p, h / G]; the first
+// prefix_len keys lie in the pages of the prefix table for every sequence, the
+// others in the sequence's own table. lens[b] <= 0: zeros.
+//
+// The softmax over both parts is joined from partials (m, l, O per row and part
+// of its keys: maximum in log2 units, sum and unnormalized output against it):
+//
+//  * The prefix: the B * G query rows of a kv head are the columns of one
+//    product against its keys. Few rows (batch_units_kernel): 32 rows per
+//    workgroup, whose waves take the prefix's tiles in turn and join their
+//    results in LDS, so that a partial leaves the workgroup once; the codes go
+//    to bf16 operands in each wave's registers. Many rows (batch_prefix_kernel):
+//    128 or 256 rows per workgroup share each tile, converted to bf16 once as it is
+//    staged in LDS, in attn_tile.hpp's pipeline.
+//  * Own keys (batch_units_kernel, the other workgroups): the tiles of all
+//    sequences are dealt out in runs of equal length, so that long sequences
+//    spread over the chip and short ones do not wait for them; a wave per
+//    (run, kv head). The number of runs fits the scratch whatever the lengths,
+//    which live on the device.
+//  * A wave's tile: K and V codes and scales of 32 keys (64 at head_dim 64), one tile in
+//    registers ahead, through the wave's own LDS (no barriers): K rows are read
+//    back in the MFMA layout, V transposed by ds_read_b64_tr_b8. E4M3 codes are
+//    exact in bf16; the per-key scales are applied in fp32 to the scores and to
+//    P, which is rounded to bf16 (half a step, 2^-9 of each weight) for
+//    v_mfma_f32_32x32x16_bf16; the row sum takes the fp32 weights.
+//  * batch_merge_kernel joins the partials of a row.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_tile.hpp"
 #include "launch.hpp"
 
 namespace rth {
 namespace {
-
-// Waves of an own-key workgroup: at head_dim 256 a wave needs over 256 registers.
-template <int D>
-constexpr int kBWaves = D == 256 ? 4 : 8;
-constexpr int kBTile  = 32;   // keys per tile of a wave
-
-// Exclusive prefix sum over the wave's lanes, and the total.
-__device__ __forceinline__ int wave_exclusive_i(int v, int lane, int& total) {
-    int x = v;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const int y = __shfl_up(x, d, kWave);
-        x += lane >= d ? y : 0;
-    }
-    total = __shfl(x, kWave - 1, kWave);
-    return x - v;
-}
 
 struct BatchView {
     const uint8_t* k;
@@ -42,19 +49,14 @@ struct BatchView {
     int            prefix_blocks;
     const int*     prefix_len;
     int            num_blocks, block_shift, num_seqs, group, hkv;
-};
 
-// Own keys [from, to) of sequence b: behind the prefix, as far as its table goes.
-struct OwnKeys {
-    int from, to;
-    __device__ __forceinline__ int tiles() const {
-        return to > from ? (to - 1) / kBTile - from / kBTile + 1 : 0;
+    __device__ __forceinline__ bool is_page(int p) const { return p >= 0 && p < num_blocks; }
+    // Physical row of key `key` on page `page`.
+    __device__ __forceinline__ int64_t row(int page, int key) const {
+        return (static_cast<int64_t>(page) << block_shift) + (key & ((1 << block_shift) - 1));
     }
 };
-__device__ __forceinline__ OwnKeys own_keys(const BatchView& t, int b, int prefix) {
-    const int64_t room = static_cast<int64_t>(t.table_blocks) << t.block_shift;
-    return {prefix, static_cast<int>(min(static_cast<int64_t>(t.lens[b]), room))};
-}
+
 __device__ __forceinline__ int prefix_keys(const BatchView& t) {
     if (t.prefix_len == nullptr) {
         return 0;
@@ -63,51 +65,445 @@ __device__ __forceinline__ int prefix_keys(const BatchView& t) {
     return static_cast<int>(min(static_cast<int64_t>(max(*t.prefix_len, 0)), room));
 }
 
-// Tiles per slot such that all sequences' runs of that many tiles (the last one
-// shorter) fit in num_slots slots.
+constexpr int kHalf = 32;   // keys of one score block
+
+// Keys [from, to) of a run of tiles of n keys.
+struct Keys {
+    int from, to;
+    __device__ __forceinline__ int tiles(int n) const {
+        return to > from ? (to - 1) / n - from / n + 1 : 0;
+    }
+};
+// Sequence b's own keys: behind the prefix, as far as its table goes.
+__device__ __forceinline__ Keys own_keys(const BatchView& t, int b, int prefix) {
+    const int64_t room = static_cast<int64_t>(t.table_blocks) << t.block_shift;
+    return {prefix, static_cast<int>(min(static_cast<int64_t>(t.lens[b]), room))};
+}
+
+// Tiles per run such that all sequences' runs of that many tiles (the last one
+// of each shorter) fit in num_slots slots.
 __device__ __forceinline__ int tiles_per_slot(int total_tiles, int num_seqs, int num_slots) {
     return max(1, (total_tiles + num_slots - num_seqs - 1) / (num_slots - num_seqs));
 }
 
+// Exclusive prefix sum over the wave's lanes, and the total.
+__device__ __forceinline__ int wave_exclusive_i(int v, int lane, int& total) {
+    int x = v;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+        const int y = __shfl_up(x, d, kWave);
+        x += lane >= d ? y : 0;
+    }
+    total = __shfl(x, kWave - 1, kWave);
+    return x - v;
+}
+
+// Units of one prefix split, and how many splits have keys.
+struct PrefixRuns {
+    int per, live;
+};
+__device__ __forceinline__ PrefixRuns prefix_runs(int tiles, int num_splits, int least) {
+    const int per = max((tiles + num_splits - 1) / num_splits, least);
+    return {per, (tiles + per - 1) / per};
+}
+
+// ---- a wave against tiles of its own ------------------------------------------
+
 template <int D>
-struct BatchTile {
-    static constexpr int kPitch = D + 16;                 // bytes per row in LDS
-    static constexpr int kCpr   = D / 16;                 // 16-byte chunks per row
-    static constexpr int kRows  = kWave / kCpr;           // rows of one load
-    static constexpr int kSteps = kBTile / kRows;
-    static constexpr int kBytes = 2 * kBTile * kPitch + 2 * kBTile * 4;
+struct WaveTile {
+    static constexpr int kWaves  = D == 256 ? 4 : 8;      // of a workgroup
+    static constexpr int kN      = D == 64 ? 64 : 32;     // keys
+    static constexpr int kSub    = kN / kHalf;
+    static constexpr int kPitch  = D + 16;                // bytes per row in LDS
+    static constexpr int kCpr    = D / 16;                // 16-byte chunks per row
+    static constexpr int kRows   = kWave / kCpr;          // rows of one load
+    static constexpr int kLoads  = kN / kRows;
+    static constexpr int kBytes  = 2 * kN * kPitch + 2 * kN * 4;   // K, V, factors
+    static constexpr int kJoin   = kWaves / 2 * kHalf * (D + 2) * 4;
+    static constexpr int kLds    = kWaves * kBytes > kJoin ? kWaves * kBytes : kJoin;
 };
 
 template <int D>
-__global__ __launch_bounds__(kBWaves<D> * kWave, D == 256 ? 1 : 2) void batch_own_kernel(
-    const uint16_t* __restrict__ q, int64_t q_stride, BatchView t, float* __restrict__ partial,
-    int* __restrict__ plan, int num_slots, float scale_log2, int nqb) {
-    using T = BatchTile<D>;
-    constexpr int kKS = D / 16, kDB = D / 32;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[kBWaves<D>][T::kBytes];
+struct WaveRows {
+    using T = WaveTile<D>;
+    static constexpr int kKS = D / 16, kDB = D / 32;
+
+    const BatchView& t;
+    uint8_t*         lds;   // the wave's
+    int              lane, kvh;
+    float            scale_log2;
+    bf16x8 qf[kKS];   // k-step 2 j + e of lane (row, h): d = 32 j + 16 h + 8 e .. + 7
+    f32x16 o[kDB];
+    float  m_ref, l_run;
+    bool   start;
+
+    u32x4 kreg[T::kLoads], vreg[T::kLoads];
+    float freg[T::kSub];
+    bool  there[T::kSub];
+
+    __device__ __forceinline__ WaveRows(const BatchView& view, uint8_t* l, int ln, int kv, float sc)
+        : t(view), lds(l), lane(ln), kvh(kv), scale_log2(sc), m_ref(0.0f), l_run(0.0f), start(true) {
+#pragma unroll
+        for (int b = 0; b < kDB; ++b) {
+            o[b] = f32x16{};
+        }
+    }
+
+    __device__ __forceinline__ void load_q(const uint16_t* row) {
+        const int h = lane >> 5;
+#pragma unroll
+        for (int s = 0; s < kKS; ++s) {
+            qf[s] = *reinterpret_cast<const bf16x8*>(row + 32 * (s >> 1) + 16 * h + 8 * (s & 1));
+        }
+    }
+
+    // The table entries of tile i (one per half), in every lane.
+    __device__ __forceinline__ void entries(const int* table, int i, int to, int (&e)[T::kSub]) const {
+#pragma unroll
+        for (int u = 0; u < T::kSub; ++u) {
+            const int key = i * T::kN + u * kHalf;
+            e[u]          = key < to ? table[key >> t.block_shift] : -1;
+        }
+    }
+
+    // Loads tile i; rows outside [from, to) and on no page are zeros.
+    __device__ __forceinline__ void load(int i, const Keys& keys, const int (&e)[T::kSub]) {
+        const int     r0 = lane / T::kCpr, chunk = lane % T::kCpr;
+        const int64_t stride = static_cast<int64_t>(t.hkv) * D;
+        int64_t base[T::kSub];
+        bool    is[T::kSub];
+#pragma unroll
+        for (int u = 0; u < T::kSub; ++u) {
+            const int page = __builtin_amdgcn_readfirstlane(e[u]);
+            is[u]   = t.is_page(page);
+            base[u] = t.row(is[u] ? page : 0, i * T::kN + u * kHalf);
+            there[u] = is[u];
+        }
+        const int lo = keys.from - i * T::kN, hi = keys.to - i * T::kN;
+#pragma unroll
+        for (int s = 0; s < T::kLoads; ++s) {
+            constexpr int kPer = kHalf / T::kRows;   // loads of a half
+            const int  u  = s / kPer, r = s * T::kRows + r0;
+            const int64_t at = (base[u] + (r - u * kHalf)) * stride + static_cast<int64_t>(kvh) * D + 16 * chunk;
+            kreg[s] = u32x4{};
+            vreg[s] = u32x4{};
+            if (is[u] && r >= lo && r < hi) {
+                kreg[s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(t.k + at));
+                vreg[s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(t.v + at));
+            }
+        }
+        // Factors: lanes 0..31 of K, the others of V.
+#pragma unroll
+        for (int u = 0; u < T::kSub; ++u) {
+            const int r = u * kHalf + (lane & 31);
+            freg[u]     = 0.0f;
+            if (is[u] && r >= lo && r < hi) {
+                const int64_t at = (base[u] + (lane & 31)) * t.hkv + kvh;
+                freg[u]          = lane < 32 ? t.ks[at] * scale_log2 : t.vs[at];
+            }
+        }
+    }
+
+    __device__ __forceinline__ void stage() {
+        const int r0 = lane / T::kCpr, chunk = lane % T::kCpr;
+#pragma unroll
+        for (int s = 0; s < T::kLoads; ++s) {
+            uint8_t* at = lds + (s * T::kRows + r0) * T::kPitch + 16 * chunk;
+            *reinterpret_cast<u32x4*>(at)                      = kreg[s];
+            *reinterpret_cast<u32x4*>(at + T::kN * T::kPitch) = vreg[s];
+        }
+        float* f = reinterpret_cast<float*>(lds + 2 * T::kN * T::kPitch);
+#pragma unroll
+        for (int u = 0; u < T::kSub; ++u) {
+            f[(lane < 32 ? 0 : T::kN) + u * kHalf + (lane & 31)] = freg[u];
+        }
+    }
+
+    // The staged keys u * 32 .. + 31: they count from row lo to below hi (of the
+    // half), and for this lane's row below its own limit.
+    __device__ __forceinline__ void half(int u, int lo, int hi) {
+        const int      col = lane & 31, h = lane >> 5;
+        const uint8_t* lk = lds + u * kHalf * T::kPitch;
+        const uint8_t* lv = lk + T::kN * T::kPitch;
+        const float*   ls = reinterpret_cast<const float*>(lds + 2 * T::kN * T::kPitch) + u * kHalf;
+        f32x16 s = {};
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+            const u32x4 w = *reinterpret_cast<const u32x4*>(lk + col * T::kPitch + 32 * j + 16 * h);
+            bf16x8 a0, a1;
+            e4m3x16_to_bf16x8x2(w, a0, a1);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0, qf[2 * j], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1, qf[2 * j + 1], s, 0, 0, 0);
+            if constexpr (D == 256) {   // operand reads ahead of the marks would not fit the registers
+                if (j % 2 == 1) {
+                    pin();
+                }
+            }
+        }
+        // Register e of a lane: key 8 (e / 4) + 4 h + e % 4 of the half.
+        f32x4 vf[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 kf = *reinterpret_cast<const f32x4*>(ls + 8 * g + 4 * h);
+            vf[g]          = *reinterpret_cast<const f32x4*>(ls + T::kN + 8 * g + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[4 * g + e] = fmaf(s[4 * g + e], kf[e], -m_ref);
+            }
+        }
+        if (__any(lo > 0 || hi < kHalf)) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int r = 8 * (e >> 2) + 4 * h + (e & 3);
+                s[e]        = r >= lo && r < hi ? s[e] : -INFINITY;
+            }
+        }
+        bf16x8 p[2];
+        float  sum;
+        auto   weights = [&]() {
+            float t0 = 0.0f, t1 = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float x = __builtin_amdgcn_exp2f(s[e]);
+                ((e & 1) != 0 ? t1 : t0) += x;
+                p[e >> 3][e & 7] = static_cast<__bf16>(x * vf[e >> 2][e & 3]);
+            }
+            sum = t0 + t1;
+        };
+        weights();
+        // A new reference maximum (lazy, as in attn_tile.hpp).
+        if (__any(start || !(sum <= 0x1p20f))) {
+            float top = s[0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) {
+                top = fmaxf(top, s[e]);
+            }
+            top               = wave_xor_max(top, 32);
+            const float up    = start ? (top == -INFINITY ? 0.0f : top) : fmaxf(top, 0.0f);
+            const float alpha = start ? 1.0f : __builtin_amdgcn_exp2f(-up);
+            m_ref += up;
+            l_run *= alpha;
+#pragma unroll
+            for (int b = 0; b < kDB; ++b) {
+                o[b] *= alpha;
+            }
+            s -= up;
+            weights();
+            start = false;
+        }
+        l_run += sum;
+        // V^T: lane (d, h), the keys of p: 16 c + 4 h + 0..3 and 16 c + 8 + 4 h + 0..3. A
+        // group of 16 lanes reads eight keys' 16 d and gets them transposed: lane i
+        // points at eight d of key i / 2.
+        typedef int i32x2 __attribute__((ext_vector_type(2)));
+        typedef __attribute__((address_space(3))) i32x2* LdsPtr;
+        const int l16 = lane & 15, rr = l16 >> 1;
+        const uint8_t* vp = lv + (4 * h + (rr & 3) + 8 * (rr >> 2)) * T::kPitch +
+                            16 * ((lane >> 4) & 1) + 8 * (l16 & 1);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int b = 0; b < kDB; ++b) {
+                const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                    (LdsPtr)const_cast<uint8_t*>(vp + 16 * c * T::kPitch + 32 * b));
+                const u32x2 x = {static_cast<uint32_t>(w.x), static_cast<uint32_t>(w.y)};
+                o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(e4m3x8_to_bf16x8(x), p[c], o[b], 0, 0, 0);
+                if constexpr (D == 256) {
+                    if (b % 4 == 3) {
+                        pin();
+                    }
+                }
+            }
+        }
+    }
+
+    // Tiles first, first + step, .. below last over keys [from, to) of a
+    // table; this lane's row sees those below `end`.
+    __device__ __forceinline__ void run(const int* table, const Keys& keys, int first, int last,
+                                        int step, int end) {
+        if (first >= last) {
+            return;
+        }
+        int e[T::kSub], next[T::kSub];
+        entries(table, first, keys.to, e);
+        entries(table, first + step, first + step < last ? keys.to : 0, next);
+        load(first, keys, e);
+        for (int i = first; i < last; i += step) {
+            bool is[T::kSub];
+#pragma unroll
+            for (int u = 0; u < T::kSub; ++u) {
+                is[u] = there[u];
+                e[u]  = next[u];
+            }
+            stage();
+            if (i + 2 * step < last) {
+                entries(table, i + 2 * step, keys.to, next);
+            }
+            if (i + step < last) {
+                load(i + step, keys, e);
+            }
+#pragma unroll
+            for (int u = 0; u < T::kSub; ++u) {
+                const int key0 = i * T::kN + u * kHalf;
+                if (is[u] && key0 < keys.to && key0 + kHalf > keys.from) {
+                    half(u, keys.from - key0, min(keys.to, end) - key0);
+                }
+            }
+        }
+    }
+
+    // m, l and O of this lane's row to `rows` partials at `part`, row `row`.
+    __device__ __forceinline__ void write(float* part, int64_t rows, int64_t row, bool has) const {
+        const int   h = again(lane) >> 5;
+        const float l = wave_xor_sum(l_run, 32);
+        if (!has) {
+            return;
+        }
+        if (h == 0) {
+            part[row]        = l == 0.0f ? -INFINITY : m_ref;
+            part[rows + row] = l;
+        }
+        float* po = part + 2 * rows + row * D + 4 * h;
+#pragma unroll
+        for (int b = 0; b < kDB; ++b) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 x = {o[b][4 * g], o[b][4 * g + 1], o[b][4 * g + 2], o[b][4 * g + 3]};
+                *reinterpret_cast<f32x4_a4*>(po + 32 * b + 8 * g) = x;
+            }
+        }
+    }
+
+    // Joins the results of the workgroup's waves into wave 0's, by halves:
+    // the upper half of the waves left hands over (area: what `all` points at).
+    __device__ __forceinline__ void join(float* all, int wave) {
+        l_run = wave_xor_sum(l_run, 32);
+        float mine = l_run == 0.0f ? -INFINITY : m_ref;
+#pragma unroll
+        for (int n = T::kWaves / 2; n > 0; n >>= 1) {
+            __syncthreads();   // tiles, or the step before, are done with
+            // A wave's area: [D / 4 + 1][64 lanes] quads of floats, m and l last.
+            float* a = all + (wave % n) * kHalf * (D + 2);
+            if (wave >= n && wave < 2 * n) {
+#pragma unroll
+                for (int b = 0; b < kDB; ++b) {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const f32x4 x = {o[b][4 * g], o[b][4 * g + 1], o[b][4 * g + 2], o[b][4 * g + 3]};
+                        *reinterpret_cast<f32x4*>(a + ((b * 4 + g) * kWave + lane) * 4) = x;
+                    }
+                }
+                if (lane < 32) {
+                    a[kHalf * D + lane]         = mine;
+                    a[kHalf * D + kHalf + lane] = l_run;
+                }
+            }
+            __syncthreads();
+            if (wave < n) {
+                const float m1 = a[kHalf * D + (lane & 31)], l1 = a[kHalf * D + kHalf + (lane & 31)];
+                float top = fmaxf(mine, m1);
+                if (m1 != m1) {
+                    top = m1;
+                }
+                const float f0 = mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - top);
+                const float f1 = m1 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m1 - top);
+                l_run = f0 * l_run + f1 * l1;
+                mine  = top;
+#pragma unroll
+                for (int b = 0; b < kDB; ++b) {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const f32x4 x = *reinterpret_cast<const f32x4*>(a + ((b * 4 + g) * kWave + lane) * 4);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            o[b][4 * g + i] = f0 * o[b][4 * g + i] + f1 * x[i];
+                        }
+                    }
+                }
+            }
+        }
+        m_ref = mine;
+        l_run *= 0.5f;   // write() adds both halves' lanes
+    }
+};
+
+// How a launch is split. Prefix: splits of the keys for each block of rows;
+// own keys: slots of runs.
+struct BatchPlan {
+    int q_blocks;      // blocks of 32 q heads of a kv head
+    int slots;
+    int splits;        // of the prefix
+    int row_blocks;    // of the prefix's rows, of a kv head
+    int tile_waves;    // 0: batch_units_kernel takes the prefix, else the waves of batch_prefix_kernel
+};
+
+constexpr int kUnitTiles = 4;   // least tiles of a prefix split of batch_units_kernel
+
+// Workgroups: first (kv head, block of 32 rows, split) of the prefix, then
+// (slot, group of units) of the own keys.
+template <int D>
+__global__ __launch_bounds__(WaveTile<D>::kWaves * kWave, D == 256 ? 1 : 2) void batch_units_kernel(
+    const uint16_t* __restrict__ q, int64_t q_stride, BatchView t, float* __restrict__ own,
+    int* __restrict__ plan, float* __restrict__ shared, BatchPlan bp, int prefix_wgs,
+    float scale_log2) {
+    using T = WaveTile<D>;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
 
     const int tid  = static_cast<int>(threadIdx.x);
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int lane = tid & (kWave - 1);
-    const int col = lane & 31, h = lane >> 5;
-    const int slot = static_cast<int>(blockIdx.x);
-    const int unit = static_cast<int>(blockIdx.y) * kBWaves<D> + wave;   // (kv head, block of q heads)
-    if (unit >= t.hkv * nqb) {
+    const int col  = lane & 31;
+    const int hq   = t.hkv * t.group;
+    int       bid  = static_cast<int>(blockIdx.x);
+    const int prefix = prefix_keys(t);
+    uint8_t*  mine   = lds + wave * T::kBytes;
+
+    if (bid < prefix_wgs) {
+        const int tiles = (prefix + T::kN - 1) / T::kN;
+        const PrefixRuns runs = prefix_runs(tiles, bp.splits, kUnitTiles);
+        const int at = uniform(bid / t.hkv), kvh = bid - at * t.hkv;
+        const int split = uniform(at / bp.row_blocks), rb = at - split * bp.row_blocks;
+        if (split >= runs.live) {
+            return;
+        }
+        const int rows = t.num_seqs * t.group;
+        const int row  = min(rb * 32 + col, rows - 1);
+        const int b = row / t.group, head = kvh * t.group + (row - b * t.group);
+        WaveRows<D> w(t, mine, lane, kvh, scale_log2);
+        w.load_q(q + b * q_stride + static_cast<int64_t>(head) * D);
+        const int first = split * runs.per;
+        w.run(t.prefix_table, Keys{0, prefix}, first + wave, min(first + runs.per, tiles), T::kWaves,
+              t.lens[b]);
+        w.join(reinterpret_cast<float*>(lds), wave);
+        if (wave == 0) {
+            const int64_t all = static_cast<int64_t>(bp.splits) * t.num_seqs * hq;
+            const int     r2 = rb * 32 + (again(lane) & 31), b2 = r2 / t.group;
+            w.write(shared, all,
+                    (static_cast<int64_t>(split) * t.num_seqs + b2) * hq + kvh * t.group + (r2 - b2 * t.group),
+                    r2 < rows);
+        }
         return;
     }
-    const int kvh = unit / nqb, qb = unit % nqb;
+    bid -= prefix_wgs;
+    const int units  = t.hkv * bp.q_blocks;
+    const int groups = (units + T::kWaves - 1) / T::kWaves;
+    const int slot = uniform(bid / groups), unit = (bid - slot * groups) * T::kWaves + wave;
+    if (unit >= units) {
+        return;
+    }
+    const int kvh = uniform(unit / bp.q_blocks), qb = unit - kvh * bp.q_blocks;
 
-    const int prefix = prefix_keys(t);
-    int       total  = 0;
+    // Which run of which sequence this slot is. Slot 0 writes the plan down.
+    int total = 0;
     for (int b0 = 0; b0 < t.num_seqs; b0 += kWave) {
         const int b = b0 + lane;
-        total += wave_sum_i(b < t.num_seqs ? own_keys(t, b, prefix).tiles() : 0);
+        total += wave_sum_i(b < t.num_seqs ? own_keys(t, b, prefix).tiles(T::kN) : 0);
     }
-    const int per = tiles_per_slot(total, t.num_seqs, num_slots);
+    const int per = tiles_per_slot(total, t.num_seqs, bp.slots);
     int seq = -1, run = 0, base = 0;
     for (int b0 = 0; b0 < t.num_seqs; b0 += kWave) {
         const int b    = b0 + lane;
-        const int runs = b < t.num_seqs ? (own_keys(t, b, prefix).tiles() + per - 1) / per : 0;
+        const int runs = b < t.num_seqs ? (own_keys(t, b, prefix).tiles(T::kN) + per - 1) / per : 0;
         int       sum;
         const int before = base + wave_exclusive_i(runs, lane, sum);
         const uint64_t hit = __ballot(slot >= before && slot < before + runs);
@@ -128,179 +524,39 @@ __global__ __launch_bounds__(kBWaves<D> * kWave, D == 256 ? 1 : 2) void batch_ow
     if (seq < 0) {
         return;
     }
-    seq                = __builtin_amdgcn_readfirstlane(seq);
-    run                = __builtin_amdgcn_readfirstlane(run);
-    const OwnKeys keys = own_keys(t, seq, prefix);
-    const int t0 = keys.from / kBTile + run * per;
-    const int t1 = min(t0 + per, (keys.to - 1) / kBTile + 1);
-    const int* table = t.tables + static_cast<int64_t>(seq) * t.table_blocks;
-
-    const int hq      = t.hkv * t.group;
-    const int my_head = kvh * t.group + min(qb * 32 + col, t.group - 1);
-    const uint16_t* qr = q + seq * q_stride + static_cast<int64_t>(my_head) * D;
-    bf16x8 qf[kKS];   // k-step 2 j + e of lane (row, h): d = 32 j + 16 h + 8 e .. + 7
-#pragma unroll
-    for (int s = 0; s < kKS; ++s) {
-        qf[s] = *reinterpret_cast<const bf16x8*>(qr + 32 * (s >> 1) + 16 * h + 8 * (s & 1));
-    }
-
-    uint8_t* lk = lds[wave];
-    uint8_t* lv = lk + kBTile * T::kPitch;
-    float*   ls = reinterpret_cast<float*>(lv + kBTile * T::kPitch);
-    const int     lrow = lane / T::kCpr, lchunk = lane % T::kCpr;
-    const int64_t stride = static_cast<int64_t>(t.hkv) * D;
-
-    f32x16 o[kDB];
-#pragma unroll
-    for (int b = 0; b < kDB; ++b) {
-        o[b] = f32x16{};
-    }
-    float m_ref = 0.0f, l_run = 0.0f;
-    bool  start = true;
-    for (int i = t0; i < t1; ++i) {
-        const int key0 = i * kBTile;
-        const int page = table[key0 >> t.block_shift];
-        if (page < 0 || page >= t.num_blocks) {
-            continue;
-        }
-        const int64_t row0 = (static_cast<int64_t>(page) << t.block_shift) +
-                             (key0 & ((1 << t.block_shift) - 1));
-        const int lo = max(keys.from - key0, 0), hi = min(keys.to - key0, kBTile);   // rows that count
-#pragma unroll
-        for (int s = 0; s < T::kSteps; ++s) {
-            const int  r    = s * T::kRows + lrow;
-            const bool live = r >= lo && r < hi;
-            const int64_t at = (row0 + r) * stride + static_cast<int64_t>(kvh) * D + 16 * lchunk;
-            u32x4 kx = {}, vx = {};
-            if (live) {
-                kx = *reinterpret_cast<const u32x4*>(t.k + at);
-                vx = *reinterpret_cast<const u32x4*>(t.v + at);
-            }
-            *reinterpret_cast<u32x4*>(lk + r * T::kPitch + 16 * lchunk) = kx;
-            *reinterpret_cast<u32x4*>(lv + r * T::kPitch + 16 * lchunk) = vx;
-        }
-        {
-            const bool    live = col >= lo && col < hi;
-            const int64_t at   = (row0 + col) * t.hkv + kvh;
-            ls[lane] = live ? (h == 0 ? t.ks[at] * scale_log2 : t.vs[at]) : 0.0f;
-        }
-        __builtin_amdgcn_wave_barrier();
-        f32x16 s = {};
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-            const u32x4 w = *reinterpret_cast<const u32x4*>(lk + col * T::kPitch + 32 * j + 16 * h);
-            bf16x8 a0, a1;
-            e4m3x16_to_bf16x8x2(w, a0, a1);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0, qf[2 * j], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1, qf[2 * j + 1], s, 0, 0, 0);
-        }
-        f32x4 vf[4];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const f32x4 kf = *reinterpret_cast<const f32x4*>(ls + 8 * g + 4 * h);
-            vf[g]          = *reinterpret_cast<const f32x4*>(ls + 32 + 8 * g + 4 * h);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = 8 * g + 4 * h + e;
-                s[4 * g + e] = r >= lo && r < hi ? fmaf(s[4 * g + e], kf[e], -m_ref) : -INFINITY;
-            }
-        }
-        bf16x8 p[2];
-        float  sum;
-        auto   weights = [&]() {
-            sum = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float x = __builtin_amdgcn_exp2f(s[e]);
-                sum += x;
-                p[e >> 3][e & 7] = static_cast<__bf16>(x * vf[e >> 2][e & 3]);
-            }
-        };
-        weights();
-        if (start || __any(!(sum <= 0x1p20f))) {
-            float top = s[0];
-#pragma unroll
-            for (int e = 1; e < 16; ++e) {
-                top = fmaxf(top, s[e]);
-            }
-            top               = wave_xor_max(top, 32);
-            const float up    = start ? (top == -INFINITY ? 0.0f : top) : fmaxf(top, 0.0f);
-            const float alpha = start ? 1.0f : __builtin_amdgcn_exp2f(-up);
-            m_ref += up;
-            l_run *= alpha;
-#pragma unroll
-            for (int b = 0; b < kDB; ++b) {
-                o[b] *= alpha;
-            }
-            s -= up;
-            weights();
-            start = false;
-        }
-        l_run += sum;
-        // V^T: lane (d, h), the keys of p: 16 c + 4 h + 0..3 and 16 c + 8 + 4 h + 0..3.
-        const int l16 = lane & 15, rr = l16 >> 1;
-        const uint8_t* vp = lv + (4 * h + (rr & 3) + 8 * (rr >> 2)) * T::kPitch +
-                            16 * ((lane >> 4) & 1) + 8 * (l16 & 1);
-#pragma unroll
-        for (int b = 0; b < kDB; ++b) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                typedef int i32x2 __attribute__((ext_vector_type(2)));
-                typedef __attribute__((address_space(3))) i32x2* LdsPtr;
-                const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                    (LdsPtr)const_cast<uint8_t*>(vp + 16 * c * T::kPitch + 32 * b));
-                const u32x2 u = {static_cast<uint32_t>(w.x), static_cast<uint32_t>(w.y)};
-                o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(e4m3x8_to_bf16x8(u), p[c], o[b], 0, 0, 0);
-            }
-        }
-        __builtin_amdgcn_wave_barrier();
-    }
-    l_run = wave_xor_sum(l_run, 32);
-    if (qb * 32 + col < t.group) {
-        const int64_t rows = static_cast<int64_t>(num_slots) * hq;
-        const int64_t row  = static_cast<int64_t>(slot) * hq + my_head;
-        if (h == 0) {
-            partial[row]        = start ? -INFINITY : m_ref;
-            partial[rows + row] = l_run;
-        }
-        float* po = partial + 2 * rows + row * D + 4 * h;
-#pragma unroll
-        for (int b = 0; b < kDB; ++b) {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x4 x = {o[b][4 * g], o[b][4 * g + 1], o[b][4 * g + 2], o[b][4 * g + 3]};
-                *reinterpret_cast<f32x4*>(po + 32 * b + 8 * g) = x;
-            }
-        }
-    }
+    seq             = uniform(seq);
+    run             = uniform(run);
+    const Keys keys = own_keys(t, seq, prefix);
+    const int t0 = keys.from / T::kN + run * per;
+    const int t1 = min(t0 + per, (keys.to - 1) / T::kN + 1);
+    const int head = kvh * t.group + min(qb * 32 + col, t.group - 1);
+    WaveRows<D> w(t, mine, lane, kvh, scale_log2);
+    w.load_q(q + seq * q_stride + static_cast<int64_t>(head) * D);
+    w.run(t.tables + static_cast<int64_t>(seq) * t.table_blocks, keys, t0, t1, 1, keys.to);
+    const int g2 = qb * 32 + (again(lane) & 31);
+    w.write(own, static_cast<int64_t>(bp.slots) * hq, static_cast<int64_t>(slot) * hq + kvh * t.group + g2,
+            g2 < t.group);
 }
 
-// Key tiles of one prefix split, and how many splits have keys.
-struct PrefixRuns {
-    int per, live;
-};
-template <int D>
-__device__ __forceinline__ PrefixRuns prefix_runs(int prefix, int num_splits) {
-    const int tiles = (prefix + AttnTile<D>::kN - 1) / AttnTile<D>::kN;
-    const int per   = max((tiles + num_splits - 1) / num_splits, 1);
-    return {per, (tiles + per - 1) / per};
-}
+// ---- many rows against the prefix ------------------------------------------------
 
-template <int D, int kQ>
-__global__ __launch_bounds__(kPThr, kQ == 1 && D < 256 ? 2 : 1) void batch_prefix_kernel(
+template <int D, int kW>
+__global__ __launch_bounds__(kW * kWave, D < 256 ? 2 : 1) void batch_prefix_kernel(
     const uint16_t* __restrict__ q, int64_t q_stride, BatchView t, float* __restrict__ partial,
     int num_splits, float scale_log2) {
-    using T           = AttnTile<D>;
-    constexpr int kBM    = 32 * kQ * kPW;
+    using T              = AttnTile<D>;
+    constexpr int kThr   = kW * kWave;
     constexpr int kCpr   = D / 16;         // 16-code chunks per row
-    constexpr int kCopy  = kPThr / kCpr;   // rows of one copy step
-    constexpr int kSteps = T::kN / kCopy < 1 ? 1 : T::kN / kCopy;
-    static_assert(kCopy <= T::kN, "");
-    __shared__ __attribute__((aligned(16))) uint8_t lds[2][T::kBytes];
-    __shared__ __attribute__((aligned(16))) float   fac[2][2][T::kN];
+    constexpr int kCopy  = kThr / kCpr;    // rows of one copy step
+    constexpr int kSteps = kCopy < T::kN ? T::kN / kCopy : 1;
+    constexpr bool kSome = kCopy > T::kN;  // more threads than chunks
+    __shared__ __attribute__((aligned(16))) uint8_t lds[T::kBytes];
+    __shared__ __attribute__((aligned(16))) float   fac[4][2 * T::kN];   // ring of four tiles
+    __shared__ int                                  here[4][2];          // halves that have a page
 
     const int prefix = prefix_keys(t);
-    const PrefixRuns runs  = prefix_runs<D>(prefix, num_splits);
+    const int tiles  = (prefix + T::kN - 1) / T::kN;
+    const PrefixRuns runs  = prefix_runs(tiles, num_splits, 1);
     const int split = static_cast<int>(blockIdx.y);
     if (split >= runs.live) {
         return;
@@ -310,188 +566,289 @@ __global__ __launch_bounds__(kPThr, kQ == 1 && D < 256 ? 2 : 1) void batch_prefi
     const int lane = tid & (kWave - 1);
     const int col = lane & 31, h = lane >> 5;
     const int bid = static_cast<int>(blockIdx.x);
-    const int blk = bid / t.hkv, hb = bid % t.hkv;
-    const int kvh  = (t.hkv & 7) == 0 ? (hb & 7) * (t.hkv >> 3) + (hb >> 3) : hb;
+    const int blk = uniform(bid / t.hkv), hb = bid - blk * t.hkv;
+    const int kvh  = uniform((t.hkv & 7) == 0 ? (hb & 7) * (t.hkv >> 3) + (hb >> 3) : hb);
     const int rows = t.num_seqs * t.group;
     const int hq   = t.hkv * t.group;
-    const int wr0  = blk * kBM + wave * 32 * kQ;
+    const int wr0  = (blk * kW + wave) * 32;
     const bool idle = wr0 >= rows;
-
-    int my_row[kQ], my_end[kQ];   // row, and how many prefix keys it sees
-#pragma unroll
-    for (int a = 0; a < kQ; ++a) {
-        my_row[a] = min(wr0 + 32 * a + col, rows - 1);
-        my_end[a] = min(prefix, t.lens[my_row[a] / t.group]);
-    }
-    const int tile0 = split * runs.per, tile1 = min(tile0 + runs.per, (prefix + T::kN - 1) / T::kN);
+    const int my_row = min(wr0 + col, rows - 1);
+    const int my_seq = my_row / t.group;
+    const int tile0 = split * runs.per, n_tiles = min(runs.per, tiles - tile0);
 
     const int crow = tid / kCpr, cchunk = tid % kCpr;
     const int64_t stride = static_cast<int64_t>(t.hkv) * D;
+    const int fkey = tid & (T::kN - 1);   // the key whose factor this thread loads (first 2 kN threads)
     u32x4 kreg[kSteps], vreg[kSteps];
-    float freg;
-    auto load = [&](int i) {
-        // A row past the prefix, or on a page that is not there, is zeros.
-        auto place = [&](int r, int64_t& row) {
-            const int key  = i * T::kN + r;
-            const int page = key < prefix ? t.prefix_table[key >> t.block_shift] : -1;
-            row = (static_cast<int64_t>(page) << t.block_shift) + (key & ((1 << t.block_shift) - 1));
-            return page >= 0 && page < t.num_blocks;
-        };
+    float freg = 0.0f;
+    struct Pages {
+        int e[2];
+    };
+    auto entries = [&](int i) {   // of the tile's halves, in every lane
+        Pages p;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int key = (tile0 + i) * T::kN + u * kHalf;
+            p.e[u]        = i < n_tiles && key < prefix ? t.prefix_table[key >> t.block_shift] : -1;
+        }
+        return p;
+    };
+    // Rows past the prefix, or on no page, are zeros.
+    auto place = [&](int i, const Pages& p, int r, int64_t& row) {
+        const int key  = (tile0 + i) * T::kN + r;
+        const int page = r < kHalf ? p.e[0] : p.e[1];
+        row            = t.row(page, key);
+        return key < prefix && t.is_page(page);
+    };
+    auto load = [&](const uint8_t* x, int i, const Pages& p, u32x4 (&reg)[kSteps]) {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             int64_t row;
-            kreg[s] = u32x4{};
-            vreg[s] = u32x4{};
-            if (place(s * kCopy + crow, row)) {
-                const int64_t at = row * stride + static_cast<int64_t>(kvh) * D + 16 * cchunk;
-                kreg[s] = *reinterpret_cast<const u32x4*>(t.k + at);
-                vreg[s] = *reinterpret_cast<const u32x4*>(t.v + at);
+            reg[s] = u32x4{};
+            if ((!kSome || crow < T::kN) && place(i, p, s * kCopy + crow, row)) {
+                reg[s] = *reinterpret_cast<const u32x4*>(x + row * stride + static_cast<int64_t>(kvh) * D +
+                                                         16 * cchunk);
             }
         }
-        // Factors: of K by the first kN threads, of V by the next.
-        freg = 0.0f;
+    };
+    auto load_fac = [&](int i, const Pages& p) {
         int64_t row;
-        if (tid < 2 * T::kN && place(tid % T::kN, row)) {
+        freg = 0.0f;
+        if (tid < 2 * T::kN && place(i, p, fkey, row)) {
             freg = tid < T::kN ? t.ks[row * t.hkv + kvh] * scale_log2 : t.vs[row * t.hkv + kvh];
         }
     };
-    auto store = [&](int i) {
-        uint8_t* b = lds[i & 1];
+    auto store = [&](uint32_t to, int pitch, const u32x4 (&reg)[kSteps]) {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            const int r = s * kCopy + crow;
-            bf16x8 x, y;
-            e4m3x16_to_bf16x8x2(kreg[s], x, y);
-            *reinterpret_cast<bf16x8*>(b + r * T::kKPitch + 32 * cchunk)      = x;
-            *reinterpret_cast<bf16x8*>(b + r * T::kKPitch + 32 * cchunk + 16) = y;
-            e4m3x16_to_bf16x8x2(vreg[s], x, y);
-            *reinterpret_cast<bf16x8*>(b + T::kK + r * T::kVPitch + 32 * cchunk)      = x;
-            *reinterpret_cast<bf16x8*>(b + T::kK + r * T::kVPitch + 32 * cchunk + 16) = y;
+            if (!kSome || crow < T::kN) {
+                bf16x8 x, y;
+                e4m3x16_to_bf16x8x2(reg[s], x, y);
+                uint8_t* at = lds + to + (s * kCopy + crow) * pitch + 32 * cchunk;
+                *reinterpret_cast<bf16x8*>(at)      = x;
+                *reinterpret_cast<bf16x8*>(at + 16) = y;
+            }
         }
+    };
+    auto store_fac = [&](int i, const Pages& p) {
         if (tid < 2 * T::kN) {
-            fac[i & 1][tid / T::kN][tid % T::kN] = freg;
+            fac[i & 3][tid] = freg;
+        }
+        if (tid < 2) {
+            here[i & 3][tid] = t.is_page(tid == 0 ? p.e[0] : p.e[1]) ? 1 : 0;
         }
     };
 
-    load(tile0);
-    QueryRows<D, kQ> rq;
-#pragma unroll
-    for (int a = 0; a < kQ; ++a) {
-        const int b = my_row[a] / t.group;
-        rq.load_q(a, q + b * q_stride + (static_cast<int64_t>(kvh) * t.group + (my_row[a] - b * t.group)) * D, h);
-    }
+    Pages pk = entries(0);   // of the K tile in kreg (and the factors in freg)
+    Pages pv = pk;           // of the V tile in vreg
+    Pages pn = entries(1);   // of the K tile after it
+    load(t.k, 0, pk, kreg);
+    load_fac(0, pk);
+    const int my_end = min(prefix, t.lens[my_seq]);   // keys this row sees
+    QueryRows<D, true, kW == 8> rq;
+    rq.lane = lane;
+    rq.load_q(q + my_seq * q_stride +
+              (static_cast<int64_t>(kvh) * t.group + (my_row - my_seq * t.group)) * D);
+    load(t.v, 0, pv, vreg);
     rq.clear();
-    store(tile0);
-    for (int i = tile0; i < tile1; ++i) {
-        __syncthreads();
-        if (i + 1 < tile1) {
-            load(i + 1);
+    store(T::k_at(0), T::kKPitch, kreg);
+    store_fac(0, pk);
+    {   // The first step multiplies zero weights with the "tile before".
+        const u32x4 zero[kSteps] = {};
+        store(T::v_at(1), T::kVPitch, zero);
+    }
+    pk = pn;
+    pn = entries(2);
+    if (n_tiles > 1) {
+        load(t.k, 1, pk, kreg);
+        load_fac(1, pk);
+    }
+    __syncthreads();
+    const int key0 = tile0 * T::kN;
+    // Halves with keys; a half that reaches past w_end is masked.
+    const int mine = idle ? -1 : (min(prefix - key0, n_tiles * T::kN) + kHalf - 1) / kHalf;
+    int       w_end;
+    {
+        int m = my_end;
+#pragma unroll
+        for (int d = 1; d < kHalf; d <<= 1) {
+            m = min(m, __shfl_xor(m, d, kWave));
         }
-        if (!idle) {
-#pragma unroll
-            for (int hf = 0; hf < T::kN / 32; ++hf) {
-                const int key0 = i * T::kN + 32 * hf;
-                const int page = key0 < prefix ? t.prefix_table[key0 >> t.block_shift] : -1;
-                if (page < 0 || page >= t.num_blocks) {
-                    continue;
-                }
-                int  lim[kQ];
-                bool masked = false;
-#pragma unroll
-                for (int a = 0; a < kQ; ++a) {
-                    lim[a] = my_end[a] - 1 - key0 - 4 * h;
-                    masked = masked || my_end[a] < key0 + 32;
-                }
-                rq.template half<true>(lds[i & 1], lds[i & 1] + T::kK, hf, lane, scale_log2, fac[i & 1][0],
-                                       fac[i & 1][1], __any(masked), lim);
+        w_end = __builtin_amdgcn_readfirstlane(m);
+    }
+    bool seen = false;   // a half with a page
+    if (mine > 0) {
+        rq.first_scores(lds + T::k_at(0));
+    }
+    for (int i = 0; i < n_tiles; ++i) {
+        auto half = [&](auto par, uint32_t k_at, uint32_t v_at) {
+            constexpr int kPar = decltype(par)::value;
+            const int     j    = 2 * i + kPar, at = key0 + 32 * j;
+            // (The step past the last half, all of it masked, adds that half's P V.)
+            if (j <= mine) {
+                rq.head(lds + k_at, lds + v_at);
+                const bool is  = j < mine && __builtin_amdgcn_readfirstlane(here[i & 3][kPar]) != 0;
+                const int  lim = is ? my_end - 1 - at - 4 * h : -1;
+                rq.template step<kPar>(lds + k_at, lds + v_at, scale_log2, fac[i & 3] + kPar * kHalf,
+                                       fac[i & 3] + T::kN + kPar * kHalf, is && !seen,
+                                       !is || at + 32 > w_end, lim);
+                seen = seen || is;
             }
+        };
+        half(std::integral_constant<int, 0>{}, T::k_at(i) + 32 * T::kKPitch, T::v_at(i + 1) + 32 * T::kVPitch);
+        // K(i + 1) over K(i - 1), V(i) over V(i - 2): last read before the barrier before.
+        if (i + 1 < n_tiles) {
+            store(T::k_at(i + 1), T::kKPitch, kreg);
+            store_fac(i + 1, pk);
         }
-        if (i + 1 < tile1) {
-            store(i + 1);
+        store(T::v_at(i), T::kVPitch, vreg);
+        __syncthreads();
+        pv = pk;
+        pk = pn;
+        pn = entries(i + 3);
+        if (i + 2 < n_tiles) {
+            load(t.k, i + 2, pk, kreg);
+            load_fac(i + 2, pk);
         }
+        if (i + 1 < n_tiles) {
+            load(t.v, i + 1, pv, vreg);
+        }
+        half(std::integral_constant<int, 1>{}, T::k_at(i + 1), T::v_at(i));
     }
     if (idle) {
         return;
     }
+    if (mine == 2 * n_tiles) {
+        rq.last(lds + T::v_at(n_tiles - 1) + 32 * T::kVPitch);
+    }
     // Partials: [splits, B, Hq] m, l, then O.
     const int64_t all = static_cast<int64_t>(num_splits) * t.num_seqs * hq;
+    const float   l   = wave_xor_sum(rq.l_run, 32);
+    const int     ln = again(lane), r = uniform(wr0) + (ln & 31), h2 = ln >> 5;
+    if (r < rows) {
+        const int     b   = r / again(t.group);
+        const int     g   = r - b * t.group;
+        const int64_t row = (static_cast<int64_t>(split) * t.num_seqs + b) * hq + kvh * t.group + g;
+        if (h2 == 0) {
+            partial[row]       = l == 0.0f ? -INFINITY : rq.m_ref;
+            partial[all + row] = l;
+        }
+        float* po = partial + 2 * all + row * D + 4 * h2;
 #pragma unroll
-    for (int a = 0; a < kQ; ++a) {
-        const float l = wave_xor_sum(rq.l_run[a], 32);
-        if (wr0 + 32 * a + col < rows) {
-            const int     b   = my_row[a] / t.group;
-            const int64_t row = (static_cast<int64_t>(split) * t.num_seqs + b) * hq + kvh * t.group +
-                                (my_row[a] - b * t.group);
-            if (h == 0) {
-                partial[row]       = l == 0.0f ? -INFINITY : rq.m_ref[a];
-                partial[all + row] = l;
-            }
-            float* po = partial + 2 * all + row * D + 4 * h;
+        for (int db = 0; db < D / 32; ++db) {
 #pragma unroll
-            for (int db = 0; db < D / 32; ++db) {
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x4 x = {rq.o[a][db][4 * g], rq.o[a][db][4 * g + 1],
-                                     rq.o[a][db][4 * g + 2], rq.o[a][db][4 * g + 3]};
-                    *reinterpret_cast<f32x4_a4*>(po + 32 * db + 8 * g) = x;
-                }
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 x = {rq.o[db][4 * g], rq.o[db][4 * g + 1], rq.o[db][4 * g + 2],
+                                 rq.o[db][4 * g + 3]};
+                *reinterpret_cast<f32x4_a4*>(po + 32 * db + 8 * g) = x;
             }
         }
     }
 }
 
-template <int D>
-__global__ __launch_bounds__(D) void batch_merge_kernel(uint16_t* __restrict__ out,
-                                                       int64_t out_stride, BatchView t,
-                                                       const float* __restrict__ own,
-                                                       const int* __restrict__ plan,
-                                                       int num_slots,
-                                                       const float* __restrict__ shared,
-                                                       int num_splits) {
-    const int hq = t.hkv * t.group;
-    const int b = static_cast<int>(blockIdx.x) / hq, head = static_cast<int>(blockIdx.x) % hq;
-    const int d = static_cast<int>(threadIdx.x);
+// ---- joining a row's partials ------------------------------------------------------
+
+constexpr int kMergeWaves = 4;
+
+// kRow: waves per row (1: a row per wave, for many rows). A group of D / 4
+// lanes takes every (groups)-th partial, four floats a lane.
+template <int D, int kRow>
+__global__ __launch_bounds__(kMergeWaves * kWave) void batch_merge_kernel(
+    uint16_t* __restrict__ out, int64_t out_stride, BatchView t, const float* __restrict__ own,
+    const int* __restrict__ plan, const float* __restrict__ shared, BatchPlan bp, int least) {
+    constexpr int kLanes  = D / 4;
+    constexpr int kGroups = kRow * kWave / kLanes;
+    __shared__ float          wsum[kMergeWaves];
+    __shared__ __attribute__((aligned(16))) float acc_s[kMergeWaves][D];
+    const int tid  = static_cast<int>(threadIdx.x);
+    const int lane = tid & (kWave - 1), wave = tid / kWave;
+    const int hq   = t.hkv * t.group;
+    const int row  = static_cast<int>(blockIdx.x) * (kMergeWaves / kRow) + wave / kRow;
+    const bool has = row < t.num_seqs * hq;
+    const int b = has ? row / hq : 0, head = has ? row % hq : 0;
     const int first = plan[2 * b], n_own = plan[2 * b + 1];
-    const int n_pre = prefix_runs<D>(prefix_keys(t), num_splits).live;
-    const int64_t own_rows = static_cast<int64_t>(num_slots) * hq;
-    const int64_t pre_rows = static_cast<int64_t>(num_splits) * t.num_seqs * hq;
-    float top = -INFINITY, l = 0.0f, acc = 0.0f;
-    auto add = [&](const float* part, int64_t rows, int64_t row) {
-        const float m = part[row];
-        if (m == -INFINITY) {
+    const int prefix = prefix_keys(t);
+    const int n_tile = bp.tile_waves != 0 ? AttnTile<D>::kN : WaveTile<D>::kN;
+    const int n_pre  = prefix_runs((prefix + n_tile - 1) / n_tile, bp.splits, least).live;
+    const int64_t own_rows = static_cast<int64_t>(bp.slots) * hq;
+    const int64_t pre_rows = static_cast<int64_t>(bp.splits) * t.num_seqs * hq;
+    const int n = t.lens[b] > 0 ? n_pre + n_own : 0;
+    // Partial s of the row: its m (l and O behind it).
+    auto part = [&](int s, int64_t& rows, int64_t& at) {
+        const bool pre = s < n_pre;
+        rows = pre ? pre_rows : own_rows;
+        at   = pre ? (static_cast<int64_t>(s) * t.num_seqs + b) * hq + head
+                   : static_cast<int64_t>(first + s - n_pre) * hq + head;
+        return pre ? shared : own;
+    };
+    float top = -INFINITY;
+    for (int s = lane; s < n; s += kWave) {
+        int64_t rows, at;
+        const float* x = part(s, rows, at);
+        top            = fmaxf(top, x[at]);
+    }
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) {
+        top = wave_xor_max(top, m);
+    }
+    const int group = (tid % (kRow * kWave)) / kLanes, d = 4 * (tid % kLanes);
+    f32x4 acc = {};
+    float l   = 0.0f;
+#pragma unroll 4
+    for (int s = group; s < n; s += kGroups) {
+        int64_t      rows, at;
+        const float* x = part(s, rows, at);
+        const float  m = x[at];
+        const f32x4  v = *reinterpret_cast<const f32x4_a4*>(x + 2 * rows + at * D + d);
+        const float  f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+        l += f * x[rows + at];
+        acc += f * v;
+    }
+    // The groups of a wave, then the waves of a row.
+#pragma unroll
+    for (int m = kLanes; m < kWave; m <<= 1) {
+        l = wave_xor_sum(l, m);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            acc[i] = wave_xor_sum(acc[i], m);
+        }
+    }
+    if constexpr (kRow > 1) {
+        if (lane < kLanes) {
+            *reinterpret_cast<f32x4*>(&acc_s[wave][d]) = acc;
+        }
+        if (lane == 0) {
+            wsum[wave] = l;
+        }
+        __syncthreads();
+        if (wave != 0) {
             return;
         }
-        const float up = fmaxf(top, m);
-        const float f0 = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - up);
-        const float f1 = m != m ? m : __builtin_amdgcn_exp2f(m - up);
-        l   = l * f0 + f1 * part[rows + row];
-        acc = acc * f0 + f1 * part[2 * rows + row * D + d];
-        top = up;
-    };
-    if (t.lens[b] > 0) {
-        for (int s = 0; s < n_pre; ++s) {
-            add(shared, pre_rows, (static_cast<int64_t>(s) * t.num_seqs + b) * hq + head);
-        }
-        for (int s = first; s < first + n_own; ++s) {
-            add(own, own_rows, static_cast<int64_t>(s) * hq + head);
+#pragma unroll
+        for (int w = 1; w < kRow; ++w) {
+            acc += *reinterpret_cast<const f32x4*>(&acc_s[w][d]);
+            l += wsum[w];
         }
     }
-    out[b * out_stride + static_cast<int64_t>(head) * D + d] =
-        f32_to_bf16_bits(l == 0.0f ? 0.0f : acc / l);
+    if (has && lane < kLanes) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        u32x2       x;
+        x.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+        x.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+        *reinterpret_cast<u32x2*>(out + b * out_stride + static_cast<int64_t>(head) * D + d) = x;
+    }
 }
 
-// How a launch is split: own slots, prefix splits.
-struct BatchPlan {
-    int slots, splits, q_blocks;
-};
-BatchPlan batch_plan(int num_seqs, int hq, int hkv, int cus) {
-    const int group = hq / hkv;
-    const int nqb   = (group + 31) / 32;
-    const int blocks = (num_seqs * group + 32 * kPW - 1) / (32 * kPW) * hkv;
+BatchPlan batch_plan(int num_seqs, int hq, int hkv, int head_dim, int cus) {
+    const int group = hq / hkv, rows = num_seqs * group;
     BatchPlan p;
-    p.q_blocks = nqb;
-    p.slots    = num_seqs + std::max(8, 8 * cus / (hkv * nqb));
-    p.splits   = std::max(1, std::min(256, (2 * cus + blocks - 1) / blocks));
+    p.q_blocks   = (group + 31) / 32;
+    p.slots      = num_seqs + std::max(8, 8 * cus / (hkv * p.q_blocks));
+    p.tile_waves = rows <= 128 ? 0 : head_dim < 256 && rows > 128 ? 8 : 4;
+    const int per_block = p.tile_waves == 0 ? 32 : 32 * p.tile_waves;
+    p.row_blocks = (rows + per_block - 1) / per_block;
+    const int wgs = p.row_blocks * hkv;
+    p.splits      = std::max(1, std::min(256, (cus + wgs - 1) / wgs));
     return p;
 }
 
@@ -501,23 +858,35 @@ template <int D>
 hipError_t launch_batch(uint16_t* out, int64_t out_stride, const uint16_t* q, int64_t q_stride,
                         const BatchView& t, float* partial, const BatchPlan& p, float scale,
                         hipStream_t stream) {
+    using T                = WaveTile<D>;
     const int   hq         = t.hkv * t.group;
     const float scale_log2 = scale * kLog2e;
     int*        plan       = reinterpret_cast<int*>(partial);
     float*      own        = partial + plan_floats(t.num_seqs);
     float*      shared     = own + static_cast<std::size_t>(p.slots) * hq * (D + 2);
-    if (t.prefix_len != nullptr) {
-        const int blocks = (t.num_seqs * t.group + 32 * kPW - 1) / (32 * kPW) * t.hkv;
-        batch_prefix_kernel<D, 1><<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(p.splits)),
-                                    kPThr, 0, stream>>>(q, q_stride, t, shared, p.splits, scale_log2);
+    const bool  some       = t.prefix_len != nullptr;
+    if (some && p.tile_waves != 0) {
+        const dim3 grid(static_cast<unsigned>(p.row_blocks * t.hkv), static_cast<unsigned>(p.splits));
+        if constexpr (D < 256) {
+            batch_prefix_kernel<D, 8><<<grid, 8 * kWave, 0, stream>>>(q, q_stride, t, shared, p.splits, scale_log2);
+        } else {
+            batch_prefix_kernel<D, 4><<<grid, 4 * kWave, 0, stream>>>(q, q_stride, t, shared, p.splits, scale_log2);
+        }
     }
     const int units = t.hkv * p.q_blocks;
-    batch_own_kernel<D><<<dim3(static_cast<unsigned>(p.slots),
-                               static_cast<unsigned>((units + kBWaves<D> - 1) / kBWaves<D>)),
-                          kBWaves<D> * kWave, 0, stream>>>(q, q_stride, t, own, plan, p.slots, scale_log2,
-                                                        p.q_blocks);
-    batch_merge_kernel<D><<<dim3(static_cast<unsigned>(t.num_seqs * hq)), D, 0, stream>>>(
-        out, out_stride, t, own, plan, p.slots, shared, p.splits);
+    const int pre   = some && p.tile_waves == 0 ? p.row_blocks * t.hkv * p.splits : 0;
+    const int wgs   = pre + p.slots * ((units + T::kWaves - 1) / T::kWaves);
+    batch_units_kernel<D><<<dim3(static_cast<unsigned>(wgs)), T::kWaves * kWave, 0, stream>>>(
+        q, q_stride, t, own, plan, shared, p, pre, scale_log2);
+    const int rows  = t.num_seqs * hq;
+    const int least = p.tile_waves == 0 ? kUnitTiles : 1;
+    if (rows >= 1024) {
+        batch_merge_kernel<D, 1><<<dim3(static_cast<unsigned>((rows + kMergeWaves - 1) / kMergeWaves)),
+                                   kMergeWaves * kWave, 0, stream>>>(out, out_stride, t, own, plan, shared, p, least);
+    } else {
+        batch_merge_kernel<D, kMergeWaves><<<dim3(static_cast<unsigned>(rows)), kMergeWaves * kWave, 0, stream>>>(
+            out, out_stride, t, own, plan, shared, p, least);
+    }
     return hipGetLastError();
 }
 
@@ -525,7 +894,7 @@ hipError_t launch_batch(uint16_t* out, int64_t out_stride, const uint16_t* q, in
 
 std::size_t batch_scratch_floats(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
                                  int cus) {
-    const BatchPlan p = batch_plan(num_seqs, num_q_heads, num_kv_heads, cus);
+    const BatchPlan p = batch_plan(num_seqs, num_q_heads, num_kv_heads, head_dim, cus);
     return plan_floats(num_seqs) +
            (static_cast<std::size_t>(p.slots) + static_cast<std::size_t>(p.splits) * num_seqs) *
                num_q_heads * (head_dim + 2);
@@ -543,7 +912,7 @@ hipError_t flash_batch_launch(uint16_t* out, int64_t out_stride, const uint16_t*
     if (e != hipSuccess) {
         return e;
     }
-    const BatchPlan p = batch_plan(num_seqs, num_q_heads, num_kv_heads, cus);
+    const BatchPlan p = batch_plan(num_seqs, num_q_heads, num_kv_heads, head_dim, cus);
     const BatchView t{k, v, k_scale, v_scale, block_tables, table_blocks, lens, prefix_table,
                       prefix_blocks, prefix_len, num_blocks, block_shift, num_seqs,
                       num_q_heads / num_kv_heads, num_kv_heads};

@@ -5,21 +5,18 @@
 // k[u, h / G]) * v[u, h / G], from the bf16 K and V rows themselves (no cache).
 //
 //  * Rows: the G q heads of a kv head are packed token by token (row r of a
-//    sequence: token r / G, head r % G), 32 kQ rows per wave, four waves per
+//    sequence: token r / G, head r % G), 32 rows per wave, four or eight waves per
 //    workgroup. A workgroup finds its (sequence, row block) itself: block w in
 //    order of the block's index within its sequence, longest first, so that the
 //    last workgroups to start are short ones, whatever mix of lengths the batch
 //    holds; no plan, no workspace and one launch.
-//  * Keys in tiles of 64 (32 at head_dim 256), K and V rows through registers into two LDS buffers (the next tile's
-//    loads run under this tile's products).
-//  * S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16_bf16: a lane owns
-//    a query row, so the softmax needs no lane exchange but for a new maximum; P^T
-//    goes from the score registers into the second product as it is: the V^T
-//    operand is read (ds_read_b64_tr_b16) in the scores' key order.
-//  * Softmax in base 2 with a lazy reference maximum in fp32; P is rounded to
-//    bf16 (half a step, 2^-9 of each weight) for the matrix product, the row
-//    sum is taken from the fp32 values.
+//  * Keys in tiles of 64, K and V rows through registers into two LDS buffers
+//    each: the loads of K(i + 2) and V(i + 1) run under the products of tiles i and i + 1,
+//    with one barrier per tile.
+//  * The tile loop is attn_tile.hpp's: softmax of half a tile under the
+//    products of its neighbours.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_tile.hpp"
 #include "launch.hpp"
@@ -27,20 +24,20 @@
 namespace rth {
 namespace {
 
-// Which (sequence, block of `bm` rows) workgroup w of a kv head takes: blocks
-// in descending order of their index j within the sequence (their work grows
-// with j), within one j in order of the sequences. nblk[b]: blocks of sequence
-// b, in LDS. False: w is past the last block.
+// Which (sequence, block of rows) workgroup w of a kv head takes: blocks in
+// descending order of their index j within the sequence (their work grows with
+// j), within one j in order of the sequences. blocks(b0): the blocks of sequence
+// b0 + lane. False: w is past the last block.
 struct BlockOf {
     int seq, j;
 };
-__device__ __forceinline__ bool find_block(int w, const int* nblk, int num_seqs, int lane,
-                                           BlockOf& at) {
+template <typename F>
+__device__ __forceinline__ bool find_block(int w, int num_seqs, F blocks, BlockOf& at) {
     // blocks with index >= t
     auto from = [&](int t) {
         int n = 0;
-        for (int b = lane; b < num_seqs; b += kWave) {
-            n += max(0, nblk[b] - t);
+        for (int b0 = 0; b0 < num_seqs; b0 += kWave) {
+            n += max(0, blocks(b0) - t);
         }
         return __builtin_amdgcn_readfirstlane(wave_sum_i(n));
     };
@@ -65,8 +62,7 @@ __device__ __forceinline__ bool find_block(int w, const int* nblk, int num_seqs,
     }
     int rank = w - above;   // among the sequences with more than lo blocks
     for (int b0 = 0; b0 < num_seqs; b0 += kWave) {
-        const int      b    = b0 + lane;
-        const bool     mine = b < num_seqs && nblk[b] > lo;
+        const bool     mine = blocks(b0) > lo;
         const uint64_t m    = __ballot(mine);
         const int      n    = __popcll(m);
         if (rank < n) {
@@ -79,20 +75,20 @@ __device__ __forceinline__ bool find_block(int w, const int* nblk, int num_seqs,
     return false;
 }
 
-template <int D, int kQ>
-__global__ __launch_bounds__(kPThr, kQ == 1 && D < 256 ? 2 : 1) void flash_packed_kernel(
+template <int D, int kW>   // kW waves of 32 rows
+__global__ __launch_bounds__(kW * kWave, D < 256 ? 2 : 1) void flash_packed_kernel(
     uint16_t* __restrict__ out, const uint16_t* __restrict__ q, const uint16_t* __restrict__ k,
     const uint16_t* __restrict__ v, const int* __restrict__ cu, int num_seqs, int num_rows,
     int64_t out_stride, int64_t q_stride, int64_t k_stride, int64_t v_stride, int group, int hkv,
     float scale_log2) {
-    using T           = AttnTile<D>;
-    constexpr int kPN = T::kN;
-    constexpr int kBM = 32 * kQ * kPW;
-    constexpr int kCpr   = D / 8;          // 16-byte chunks per row
-    constexpr int kCopy  = kPThr / kCpr;   // rows of one copy step
-    constexpr int kSteps = kPN / kCopy;
-    constexpr int kTiles = 2 * T::kBytes > 4 * kMaxBatchSeqs ? 2 * T::kBytes : 4 * kMaxBatchSeqs;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[kTiles];
+    using T              = AttnTile<D>;
+    constexpr int kThr   = kW * kWave;
+    constexpr int kBM    = 32 * kW;
+    constexpr int kCpr   = D / 8;         // 16-byte chunks per row
+    constexpr int kCopy  = kThr / kCpr;   // rows of one copy step
+    constexpr int kSteps = T::kN / kCopy;
+    static_assert(T::kBytes >= 4 * kMaxBatchSeqs, "the block counts of a batch fit the tiles");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[T::kBytes];
 
     const int tid  = static_cast<int>(threadIdx.x);
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -106,15 +102,26 @@ __global__ __launch_bounds__(kPThr, kQ == 1 && D < 256 ? 2 : 1) void flash_packe
     const int kvh = (hkv & 7) == 0 ? (hb & 7) * (hkv >> 3) + (hb >> 3) : hb;
 
     BlockOf at;
+    bool    found;
     {
-        int* nblk = reinterpret_cast<int*>(lds);
-        for (int b = tid; b < num_seqs; b += kPThr) {
-            const int n = clamp_rows(cu[b + 1], num_rows) - clamp_rows(cu[b], num_rows);
-            nblk[b] = static_cast<int>((static_cast<int64_t>(max(n, 0)) * group + kBM - 1) / kBM);
+        auto count = [&](int b) {
+            const int n = b < num_seqs
+                              ? clamp_rows(cu[b + 1], num_rows) - clamp_rows(cu[b], num_rows) : 0;
+            return static_cast<int>((static_cast<int64_t>(max(n, 0)) * group + kBM - 1) / kBM);
+        };
+        if (num_seqs <= kWave) {   // every wave by itself, from registers
+            const int n = count(lane);
+            found       = find_block(w, num_seqs, [&](int) { return n; }, at);
+        } else {
+            int* nblk = reinterpret_cast<int*>(lds);
+            for (int b = tid; b < num_seqs; b += kThr) {
+                nblk[b] = count(b);
+            }
+            __syncthreads();
+            found = find_block(
+                w, num_seqs, [&](int b0) { return b0 + lane < num_seqs ? nblk[b0 + lane] : 0; }, at);
+            __syncthreads();
         }
-        __syncthreads();
-        const bool found = find_block(w, nblk, num_seqs, lane, at);
-        __syncthreads();
         if (!found) {
             return;
         }
@@ -125,115 +132,118 @@ __global__ __launch_bounds__(kPThr, kQ == 1 && D < 256 ? 2 : 1) void flash_packe
     const int n     = clamp_rows(cu[seq + 1], num_rows) - first;
     const int rows  = n * group;
     const int r0    = j * kBM;
-    const int n_tiles = (min(r0 + kBM, rows) - 1) / group / kPN + 1;
+    const int n_tiles = (min(r0 + kBM, rows) - 1) / group / T::kN + 1;
 
-    // Rows of this lane; past the sequence's last they repeat it and store nothing.
-    int my_row[kQ], my_tok[kQ];
-    const int wr0 = r0 + wave * 32 * kQ;
-#pragma unroll
-    for (int a = 0; a < kQ; ++a) {
-        my_row[a] = min(wr0 + 32 * a + col, rows - 1);
-        my_tok[a] = my_row[a] / group;
-    }
-    // The wave's first and last token, for the tiles it masks or skips.
+    // This lane's row; past the sequence's last it repeats that and stores nothing.
+    const int wr0    = r0 + wave * 32;
+    const int my_row = min(wr0 + col, rows - 1);
+    const int my_tok = my_row / group;
+    // The wave's first token (halves past it are masked), and its halves.
     const int w_first = min(wr0, rows - 1) / group;
-    const int w_last  = min(wr0 + 32 * kQ - 1, rows - 1) / group;
-    const bool idle   = wr0 >= rows;
+    const int mine    = wr0 < rows ? (min(wr0 + 31, rows - 1) / group) / 32 + 1 : -1;
 
-    const int64_t row0 = first;
-    const uint16_t* kh = k + row0 * k_stride + static_cast<int64_t>(kvh) * D;
-    const uint16_t* vh = v + row0 * v_stride + static_cast<int64_t>(kvh) * D;
-    const int crow = tid / kCpr, cchunk = tid % kCpr;
+    const int64_t   row0 = first;
+    const uint16_t* kh   = k + row0 * k_stride + static_cast<int64_t>(kvh) * D;
+    const uint16_t* vh   = v + row0 * v_stride + static_cast<int64_t>(kvh) * D;
+    const int       crow = tid / kCpr, cchunk = tid % kCpr;
     u32x4 kreg[kSteps], vreg[kSteps];
-    auto load = [&](int i) {
+    // A row past the sequence's last repeats it: every key past a row's own is masked.
+    auto load = [&](const uint16_t* x, int64_t stride, int i, u32x4 (&reg)[kSteps]) {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            const int64_t r = min(i * kPN + s * kCopy + crow, n - 1);
-            kreg[s] = *reinterpret_cast<const u32x4*>(kh + r * k_stride + 8 * cchunk);
-            vreg[s] = *reinterpret_cast<const u32x4*>(vh + r * v_stride + 8 * cchunk);
+            const int64_t r = min(i * T::kN + s * kCopy + crow, n - 1);
+            reg[s]          = *reinterpret_cast<const u32x4*>(x + r * stride + 8 * cchunk);
         }
     };
-    auto store = [&](int i) {
-        uint8_t* b = lds + (i & 1) * T::kBytes;
+    auto store = [&](uint32_t to, int pitch, const u32x4 (&reg)[kSteps]) {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            const int r = s * kCopy + crow;
-            *reinterpret_cast<u32x4*>(b + r * T::kKPitch + 16 * cchunk)         = kreg[s];
-            *reinterpret_cast<u32x4*>(b + T::kK + r * T::kVPitch + 16 * cchunk) = vreg[s];
+            *reinterpret_cast<u32x4*>(lds + to + (s * kCopy + crow) * pitch + 16 * cchunk) = reg[s];
         }
     };
 
-    load(0);
-    QueryRows<D, kQ> rq;
-#pragma unroll
-    for (int a = 0; a < kQ; ++a) {
-        const int64_t t = my_tok[a];
-        rq.load_q(a, q + (row0 + t) * q_stride +
-                         (static_cast<int64_t>(kvh) * group + (my_row[a] - my_tok[a] * group)) * D, h);
-    }
+    load(kh, k_stride, 0, kreg);
+    QueryRows<D, false, kW == 8> rq;
+    rq.lane = lane;
+    rq.load_q(q + (row0 + my_tok) * q_stride +
+              (static_cast<int64_t>(kvh) * group + (my_row - my_tok * group)) * D);
+    load(vh, v_stride, 0, vreg);
     rq.clear();
-    store(0);
-
-    for (int i = 0; i < n_tiles; ++i) {
-        __syncthreads();
-        if (i + 1 < n_tiles) {
-            load(i + 1);
-        }
-        const uint8_t* kb = lds + (i & 1) * T::kBytes;
-        const uint8_t* vb = kb + T::kK;
-        if (!idle && i * kPN <= w_last) {
-#pragma unroll
-            for (int hf = 0; hf < kPN / 32; ++hf) {
-                const int key0 = i * kPN + 32 * hf;
-                int       lim[kQ];
-#pragma unroll
-                for (int a = 0; a < kQ; ++a) {
-                    lim[a] = my_tok[a] - key0 - 4 * h;
-                }
-                rq.template half<false>(kb, vb, hf, lane, scale_log2, nullptr, nullptr,
-                                        key0 + 31 > w_first, lim);
-            }
-        }
-        if (i + 1 < n_tiles) {
-            store(i + 1);
-        }
+    store(T::k_at(0), T::kKPitch, kreg);
+    // The first step multiplies zero weights with the "tile before".
+    {
+        const u32x4 zero[kSteps] = {};
+        store(T::v_at(1), T::kVPitch, zero);
     }
-    if (idle) {
+    if (n_tiles > 1) {
+        load(kh, k_stride, 1, kreg);
+    }
+    __syncthreads();
+    if (mine > 0) {
+        rq.first_scores(lds + T::k_at(0));
+    }
+    for (int i = 0; i < n_tiles; ++i) {
+        auto half = [&](auto par, uint32_t k_at, uint32_t v_at) {
+            constexpr int kPar = decltype(par)::value;
+            const int     j    = 2 * i + kPar;
+            // (The step past the last half, all of it masked, adds that half's P V.)
+            if (j <= mine) {
+                rq.head(lds + k_at, lds + v_at);
+                rq.template step<kPar>(lds + k_at, lds + v_at, scale_log2, nullptr, nullptr, j == 0,
+                                       32 * j + 31 > w_first, my_tok - 32 * j - 4 * h);
+            }
+        };
+        half(std::integral_constant<int, 0>{}, T::k_at(i) + 32 * T::kKPitch, T::v_at(i + 1) + 32 * T::kVPitch);
+        // K(i + 1) over K(i - 1), V(i) over V(i - 2): last read before the barrier before.
+        if (i + 1 < n_tiles) {
+            store(T::k_at(i + 1), T::kKPitch, kreg);
+        }
+        store(T::v_at(i), T::kVPitch, vreg);
+        __syncthreads();
+        if (i + 2 < n_tiles) {
+            load(kh, k_stride, i + 2, kreg);
+        }
+        if (i + 1 < n_tiles) {
+            load(vh, v_stride, i + 1, vreg);
+        }
+        half(std::integral_constant<int, 1>{}, T::k_at(i + 1), T::v_at(i));
+    }
+    if (mine < 0) {
         return;
     }
+    if (mine == 2 * n_tiles) {
+        rq.last(lds + T::v_at(n_tiles - 1) + 32 * T::kVPitch);
+    }
+    const float inv = 1.0f / wave_xor_sum(rq.l_run, 32);
+    const int   r   = again(wr0 + col);
+    if (r < rows) {
+        const int64_t t    = r / group;
+        uint16_t*     orow = out + (row0 + t) * out_stride +
+                         (static_cast<int64_t>(kvh) * group + (r - t * group)) * D;
 #pragma unroll
-    for (int a = 0; a < kQ; ++a) {
-        const float inv = 1.0f / wave_xor_sum(rq.l_run[a], 32);
-        const int   r   = again(wr0 + 32 * a + col);
-        if (r < rows) {
-            const int64_t t = r / group;
-            uint16_t* orow = out + (row0 + t) * out_stride +
-                             (static_cast<int64_t>(kvh) * group + (r - t * group)) * D;
+        for (int b = 0; b < D / 32; ++b) {
 #pragma unroll
-            for (int b = 0; b < D / 32; ++b) {
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    u32x2 x;
-                    x.x = pack_bf16x2(rq.o[a][b][4 * g] * inv, rq.o[a][b][4 * g + 1] * inv);
-                    x.y = pack_bf16x2(rq.o[a][b][4 * g + 2] * inv, rq.o[a][b][4 * g + 3] * inv);
-                    *reinterpret_cast<u32x2*>(orow + 32 * b + 8 * g + 4 * h) = x;
-                }
+            for (int g = 0; g < 4; ++g) {
+                u32x2 x;
+                x.x = pack_bf16x2(rq.o[b][4 * g] * inv, rq.o[b][4 * g + 1] * inv);
+                x.y = pack_bf16x2(rq.o[b][4 * g + 2] * inv, rq.o[b][4 * g + 3] * inv);
+                *reinterpret_cast<u32x2*>(orow + 32 * b + 8 * g + 4 * h) = x;
             }
         }
     }
 }
 
-template <int D, int kQ>
+template <int D, int kW>
 hipError_t launch_packed(uint16_t* out, const uint16_t* q, const uint16_t* k, const uint16_t* v,
                          const int* cu, int num_seqs, int num_rows, int64_t out_stride,
                          int64_t q_stride, int64_t k_stride, int64_t v_stride, int hq, int hkv,
                          float scale, hipStream_t stream) {
-    constexpr int kBM = 32 * kQ * kPW;
+    constexpr int kBM = 32 * kW;
     const int     group = hq / hkv;
     // Most row blocks that the rows can make up in num_seqs sequences.
     const int64_t packed = static_cast<int64_t>(num_rows) * group;
     const int64_t blocks = std::min<int64_t>(packed, packed / kBM + num_seqs);
-    flash_packed_kernel<D, kQ><<<dim3(static_cast<unsigned>(blocks * hkv)), kPThr, 0, stream>>>(
+    flash_packed_kernel<D, kW><<<dim3(static_cast<unsigned>(blocks * hkv)), kW * kWave, 0, stream>>>(
         out, q, k, v, cu, num_seqs, num_rows, out_stride, q_stride, k_stride, v_stride, group, hkv,
         scale * kLog2e);
     return hipGetLastError();
@@ -246,16 +256,37 @@ hipError_t flash_packed_launch(uint16_t* out, const uint16_t* q, const uint16_t*
                                int num_rows, int64_t out_stride, int64_t q_stride,
                                int64_t k_stride, int64_t v_stride, int num_q_heads,
                                int num_kv_heads, int head_dim, float scale, hipStream_t stream) {
-#define RTH_PACKED(D, Q)                                                                          \
-    return launch_packed<D, Q>(out, q, k, v, cu_seqlens, num_seqs, num_rows, out_stride, q_stride, \
+    int        cus = 0;
+    hipError_t e   = device_cu_count(&cus);
+    if (e != hipSuccess) {
+        return e;
+    }
+    // Eight waves a workgroup (256 rows, one workgroup of two waves per SIMD: half the
+    // copies of K and V per row, and the wave priority) where there are long
+    // sequences and 1.75 workgroups per compute unit of them; else four (128 rows, two
+    // workgroups per compute unit), whose blocks waste less at the diagonal and even out
+    // better. Four / eight, us: 1 x 8192 tokens, 32 heads 552 / 495, 1 x 4096 160 / 135,
+    // 4 x 2000 156 / 145, 4 x 2000 of 16 heads 86 / 79, but 8 x 1000 94 / 95, 16 x 500
+    // 64 / 73, 1 x 2048 54 / 57, 1 x 4096 of 16 heads 99 / 103; head_dim 64 1 x 4096
+    // 114 / 100, 16 x 500 44 / 46.
+    const int64_t wide = static_cast<int64_t>(num_rows) * num_q_heads / 256;
+    const bool    eight = num_rows / num_seqs >= 1500 && 4 * wide >= 7 * static_cast<int64_t>(cus);
+#define RTH_PACKED(D, W)                                                                          \
+    return launch_packed<D, W>(out, q, k, v, cu_seqlens, num_seqs, num_rows, out_stride, q_stride, \
                                k_stride, v_stride, num_q_heads, num_kv_heads, scale, stream)
     switch (head_dim) {
         case 64:
-            RTH_PACKED(64, 1);
+            if (eight) {
+                RTH_PACKED(64, 8);
+            }
+            RTH_PACKED(64, 4);
         case 128:
-            RTH_PACKED(128, 1);
+            if (eight) {
+                RTH_PACKED(128, 8);
+            }
+            RTH_PACKED(128, 4);
         case 256:
-            RTH_PACKED(256, 1);
+            RTH_PACKED(256, 4);
         default:
             return hipErrorInvalidValue;
     }

@@ -66,6 +66,8 @@ def test_heads(hq, hkv, d):
 
 @pytest.mark.parametrize("lens,hq,hkv,d", [
     ([1500, 40], 32, 8, 128), ([2049], 16, 8, 64), ([1100, 900], 8, 4, 256), ([4100], 8, 8, 128),
+    # The eight-wave workgroups (long sequences, enough of them to fill the chip).
+    ([4200], 32, 8, 128), ([3001, 2500, 17], 28, 4, 128), ([4097], 40, 8, 64),
 ])
 def test_long(lens, hq, hkv, d):
     check(lens, hq, hkv, d, 300 + lens[0], rows=[1023, 1024, 1025])
