@@ -10,7 +10,7 @@
 // of its keys: maximum in log2 units, sum and unnormalized output against it):
 //
 //  * The prefix: the B * G query rows of a kv head are the columns of one
-//    product against its keys. Few rows (batch_units_kernel): 32 rows per
+//    product against its keys. Few rows (batch_units_kernel): 16 rows per
 //    workgroup, whose waves take the prefix's tiles in turn and join their
 //    results in LDS, so that a partial leaves the workgroup once; the codes go
 //    to bf16 operands in each wave's registers. Many rows (batch_prefix_kernel):
@@ -26,7 +26,7 @@
 //    back in the MFMA layout, V transposed by ds_read_b64_tr_b8. E4M3 codes are
 //    exact in bf16; the per-key scales are applied in fp32 to the scores and to
 //    P, which is rounded to bf16 (half a step, 2^-9 of each weight) for
-//    v_mfma_f32_32x32x16_bf16; the row sum takes the fp32 weights.
+//    the bf16 MFMA; the row sum takes the fp32 weights.
 //  * batch_merge_kernel joins the partials of a row.
 #include <algorithm>
 #include <type_traits>
@@ -111,49 +111,60 @@ __device__ __forceinline__ PrefixRuns prefix_runs(int tiles, int num_splits, int
 
 template <int D>
 struct WaveTile {
-    static constexpr int kWaves  = D == 256 ? 4 : 8;      // of a workgroup
+    static constexpr int kRowsQ  = 16;                    // query rows of a wave
     static constexpr int kN      = D == 64 ? 64 : 32;     // keys
     static constexpr int kSub    = kN / kHalf;
     static constexpr int kPitch  = D + 16;                // bytes per row in LDS
+    // V rows 16.. of a half lie this much further: the transposing reads take
+    // rows 16 apart at once, which no pitch spreads over the banks.
+    static constexpr int kSkew   = D == 64 ? 32 : D == 128 ? 16 : 64;
+    static constexpr int kVHalf  = kHalf * kPitch + kSkew;
     static constexpr int kCpr    = D / 16;                // 16-byte chunks per row
     static constexpr int kRows   = kWave / kCpr;          // rows of one load
     static constexpr int kLoads  = kN / kRows;
-    static constexpr int kBytes  = 2 * kN * kPitch + 2 * kN * 4;   // K, V, factors
-    static constexpr int kJoin   = kWaves / 2 * kHalf * (D + 2) * 4;
-    static constexpr int kLds    = kWaves * kBytes > kJoin ? kWaves * kBytes : kJoin;
+    static constexpr int kV      = kN * kPitch;           // where V, and the factors start
+    static constexpr int kF      = kV + kSub * kVHalf;
+    static constexpr int kBytes  = kF + 2 * kN * 4;
+    static constexpr int kArea   = kRowsQ * (D + 2);      // floats a wave hands over
+    template <int kW>   // waves of a workgroup
+    static constexpr int kLds = std::max(kW * kBytes, kW / 2 * kArea * 4);
 };
 
+// 16 query rows (the columns of v_mfma_f32_16x16x32_bf16, lane l: row l % 16) of a
+// wave. (With 32 and v_mfma_f32_32x32x16 the operands and sums take twice the
+// registers, so half the waves have loads in flight.)
 template <int D>
 struct WaveRows {
     using T = WaveTile<D>;
-    static constexpr int kKS = D / 16, kDB = D / 32;
+    static constexpr int kKS = D / 32, kDB = D / 16;
 
     const BatchView& t;
     uint8_t*         lds;   // the wave's
     int              lane, kvh;
     float            scale_log2;
-    bf16x8 qf[kKS];   // k-step 2 j + e of lane (row, h): d = 32 j + 16 h + 8 e .. + 7
-    f32x16 o[kDB];
+    bf16x8 qf[kKS];   // k-step 2 j + e of lane (row, g): d = 64 j + 16 g + 8 e .. + 7
+    f32x4  o[kDB];    // lane (row, g): d = 16 b + 4 g .. + 3
     float  m_ref, l_run;
     bool   start;
 
     u32x4 kreg[T::kLoads], vreg[T::kLoads];
     float freg[T::kSub];
+    int   lo[T::kSub], hi[T::kSub];   // rows of the loaded halves that count
     bool  there[T::kSub];
 
     __device__ __forceinline__ WaveRows(const BatchView& view, uint8_t* l, int ln, int kv, float sc)
         : t(view), lds(l), lane(ln), kvh(kv), scale_log2(sc), m_ref(0.0f), l_run(0.0f), start(true) {
 #pragma unroll
         for (int b = 0; b < kDB; ++b) {
-            o[b] = f32x16{};
+            o[b] = f32x4{};
         }
     }
 
     __device__ __forceinline__ void load_q(const uint16_t* row) {
-        const int h = lane >> 5;
+        const int g = lane >> 4;
 #pragma unroll
         for (int s = 0; s < kKS; ++s) {
-            qf[s] = *reinterpret_cast<const bf16x8*>(row + 32 * (s >> 1) + 16 * h + 8 * (s & 1));
+            qf[s] = *reinterpret_cast<const bf16x8*>(row + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
         }
     }
 
@@ -166,119 +177,144 @@ struct WaveRows {
         }
     }
 
-    // Loads tile i; rows outside [from, to) and on no page are zeros.
+    // Codes are read once (nontemporal) where a head's row is a whole 128-byte line;
+    // the heads' waves of a workgroup share the lines of shorter rows.
+    static __device__ __forceinline__ u32x4 codes(const uint8_t* p, uint32_t off) {
+        if constexpr (D >= 128) {
+            return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + off));
+        } else {
+            return *reinterpret_cast<const u32x4*>(p + off);
+        }
+    }
+
+    // Loads tile i. Rows outside [from, to) repeat one inside (their V is made
+    // zeros as it is staged, and their factors are).
     __device__ __forceinline__ void load(int i, const Keys& keys, const int (&e)[T::kSub]) {
-        const int     r0 = lane / T::kCpr, chunk = lane % T::kCpr;
-        const int64_t stride = static_cast<int64_t>(t.hkv) * D;
-        int64_t base[T::kSub];
-        bool    is[T::kSub];
+        const int ln = again(lane);   // (addresses: computed anew for each tile)
+        const uint32_t stride = static_cast<uint32_t>(t.hkv) * D;
+        const uint32_t r0 = static_cast<uint32_t>(ln / T::kCpr), chunk = static_cast<uint32_t>(ln % T::kCpr);
+        constexpr int  kPer = kHalf / T::kRows;   // loads of a half
 #pragma unroll
         for (int u = 0; u < T::kSub; ++u) {
-            const int page = __builtin_amdgcn_readfirstlane(e[u]);
-            is[u]   = t.is_page(page);
-            base[u] = t.row(is[u] ? page : 0, i * T::kN + u * kHalf);
-            there[u] = is[u];
-        }
-        const int lo = keys.from - i * T::kN, hi = keys.to - i * T::kN;
-#pragma unroll
-        for (int s = 0; s < T::kLoads; ++s) {
-            constexpr int kPer = kHalf / T::kRows;   // loads of a half
-            const int  u  = s / kPer, r = s * T::kRows + r0;
-            const int64_t at = (base[u] + (r - u * kHalf)) * stride + static_cast<int64_t>(kvh) * D + 16 * chunk;
-            kreg[s] = u32x4{};
-            vreg[s] = u32x4{};
-            if (is[u] && r >= lo && r < hi) {
-                kreg[s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(t.k + at));
-                vreg[s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(t.v + at));
+            const int page = uniform(e[u]), key0 = i * T::kN + u * kHalf;
+            lo[u]    = max(keys.from - key0, 0);
+            hi[u]    = min(keys.to - key0, kHalf);
+            there[u] = t.is_page(page) && lo[u] < hi[u];
+            if (!there[u]) {   // (the first page's rows, which nothing uses)
+                lo[u] = 0;
+                hi[u] = kHalf;
             }
-        }
-        // Factors: lanes 0..31 of K, the others of V.
+            const int64_t  row = t.row(there[u] ? page : 0, key0);
+            const int64_t  at  = row * stride + static_cast<int64_t>(kvh) * D;
+            const uint8_t* kp  = t.k + at;
+            const uint8_t* vp  = t.v + at;
+            if (lo[u] == 0 && hi[u] == kHalf) {
+                const uint32_t off = r0 * stride + 16u * chunk;
 #pragma unroll
-        for (int u = 0; u < T::kSub; ++u) {
-            const int r = u * kHalf + (lane & 31);
-            freg[u]     = 0.0f;
-            if (is[u] && r >= lo && r < hi) {
-                const int64_t at = (base[u] + (lane & 31)) * t.hkv + kvh;
-                freg[u]          = lane < 32 ? t.ks[at] * scale_log2 : t.vs[at];
+                for (int s = 0; s < kPer; ++s) {
+                    const uint32_t more = static_cast<uint32_t>(s * T::kRows) * stride;
+                    kreg[u * kPer + s] = codes(kp + more, off);
+                    vreg[u * kPer + s] = codes(vp + more, off);
+                }
+            } else {
+#pragma unroll
+                for (int s = 0; s < kPer; ++s) {
+                    const int      r   = min(max(s * T::kRows + static_cast<int>(r0), lo[u]), hi[u] - 1);
+                    const uint32_t off = static_cast<uint32_t>(r) * stride + 16u * chunk;
+                    kreg[u * kPer + s] = codes(kp, off);
+                    vreg[u * kPer + s] = codes(vp, off);
+                }
             }
+            // Factors: lanes 0..31 of K, the others of V.
+            const int    r = ln & 31;
+            const float* f = (ln < 32 ? t.ks : t.vs) + row * t.hkv + kvh;
+            freg[u] = f[static_cast<uint32_t>(min(max(r, lo[u]), hi[u] - 1)) * static_cast<uint32_t>(t.hkv)];
         }
     }
 
     __device__ __forceinline__ void stage() {
-        const int r0 = lane / T::kCpr, chunk = lane % T::kCpr;
-#pragma unroll
-        for (int s = 0; s < T::kLoads; ++s) {
-            uint8_t* at = lds + (s * T::kRows + r0) * T::kPitch + 16 * chunk;
-            *reinterpret_cast<u32x4*>(at)                      = kreg[s];
-            *reinterpret_cast<u32x4*>(at + T::kN * T::kPitch) = vreg[s];
-        }
-        float* f = reinterpret_cast<float*>(lds + 2 * T::kN * T::kPitch);
+        const int ln = again(lane);
+        const int r0 = ln / T::kCpr, chunk = ln % T::kCpr;
+        constexpr int kPer = kHalf / T::kRows;
+        float* f = reinterpret_cast<float*>(lds + T::kF);
 #pragma unroll
         for (int u = 0; u < T::kSub; ++u) {
-            f[(lane < 32 ? 0 : T::kN) + u * kHalf + (lane & 31)] = freg[u];
+            const bool edge = lo[u] > 0 || hi[u] < kHalf;
+            uint8_t*   at   = lds + r0 * T::kPitch + 16 * chunk;
+#pragma unroll
+            for (int s = 0; s < kPer; ++s) {
+                const int r = s * T::kRows;
+                u32x4     v = vreg[u * kPer + s];
+                if (edge && (r + r0 < lo[u] || r + r0 >= hi[u])) {
+                    v = u32x4{};
+                }
+                *reinterpret_cast<u32x4*>(at + (u * kHalf + r) * T::kPitch) = kreg[u * kPer + s];
+                *reinterpret_cast<u32x4*>(at + T::kV + u * T::kVHalf + r * T::kPitch + (r >= 16 ? T::kSkew : 0)) = v;
+            }
+            const int  r  = ln & 31;
+            const bool in = r >= lo[u] && r < hi[u];
+            f[(ln < 32 ? 0 : T::kN) + u * kHalf + r] = in ? freg[u] * (ln < 32 ? scale_log2 : 1.0f) : 0.0f;
         }
     }
 
-    // The staged keys u * 32 .. + 31: they count from row lo to below hi (of the
-    // half), and for this lane's row below its own limit.
+    // The staged keys u * 32 .. + 31, of which this lane's row sees rows lo .. hi - 1.
     __device__ __forceinline__ void half(int u, int lo, int hi) {
-        const int      col = lane & 31, h = lane >> 5;
+        const int      ln = again(lane), row = ln & 15, g = ln >> 4;
         const uint8_t* lk = lds + u * kHalf * T::kPitch;
-        const uint8_t* lv = lk + T::kN * T::kPitch;
-        const float*   ls = reinterpret_cast<const float*>(lds + 2 * T::kN * T::kPitch) + u * kHalf;
-        f32x16 s = {};
+        const uint8_t* lv = lds + T::kV + u * T::kVHalf;
+        const float*   ls = reinterpret_cast<const float*>(lds + T::kF) + u * kHalf;
+        // Register 4 a + e of a lane: key 16 a + 4 g + e of the half.
+        float s[8];
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-            const u32x4 w = *reinterpret_cast<const u32x4*>(lk + col * T::kPitch + 32 * j + 16 * h);
-            bf16x8 a0, a1;
-            e4m3x16_to_bf16x8x2(w, a0, a1);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0, qf[2 * j], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1, qf[2 * j + 1], s, 0, 0, 0);
-            if constexpr (D == 256) {   // operand reads ahead of the marks would not fit the registers
-                if (j % 2 == 1) {
-                    pin();
-                }
+        for (int a = 0; a < 2; ++a) {
+            pin();   // operand reads ahead of the marks would not fit the registers
+            f32x4 x = {};
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(lk + (16 * a + row) * T::kPitch + 64 * j + 16 * g);
+                bf16x8 a0, a1;
+                e4m3x16_to_bf16x8x2(w, a0, a1);
+                x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, qf[2 * j], x, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, qf[2 * j + 1], x, 0, 0, 0);
             }
-        }
-        // Register e of a lane: key 8 (e / 4) + 4 h + e % 4 of the half.
-        f32x4 vf[4];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const f32x4 kf = *reinterpret_cast<const f32x4*>(ls + 8 * g + 4 * h);
-            vf[g]          = *reinterpret_cast<const f32x4*>(ls + T::kN + 8 * g + 4 * h);
+            const f32x4 kf = *reinterpret_cast<const f32x4*>(ls + 16 * a + 4 * g);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                s[4 * g + e] = fmaf(s[4 * g + e], kf[e], -m_ref);
+                s[4 * a + e] = fmaf(x[e], kf[e], -m_ref);
             }
         }
         if (__any(lo > 0 || hi < kHalf)) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int r = 8 * (e >> 2) + 4 * h + (e & 3);
+            for (int e = 0; e < 8; ++e) {
+                const int r = 16 * (e >> 2) + 4 * g + (e & 3);
                 s[e]        = r >= lo && r < hi ? s[e] : -INFINITY;
             }
         }
-        bf16x8 p[2];
+        pin();
+        bf16x8 p;
         float  sum;
         auto   weights = [&]() {
-            float t0 = 0.0f, t1 = 0.0f;
+            sum = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float x = __builtin_amdgcn_exp2f(s[e]);
-                ((e & 1) != 0 ? t1 : t0) += x;
-                p[e >> 3][e & 7] = static_cast<__bf16>(x * vf[e >> 2][e & 3]);
+            for (int a = 0; a < 2; ++a) {
+                const f32x4 vf = *reinterpret_cast<const f32x4*>(ls + T::kN + 16 * a + 4 * g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = __builtin_amdgcn_exp2f(s[4 * a + e]);
+                    sum += x;
+                    p[4 * a + e] = static_cast<__bf16>(x * vf[e]);
+                }
             }
-            sum = t0 + t1;
         };
         weights();
         // A new reference maximum (lazy, as in attn_tile.hpp).
         if (__any(start || !(sum <= 0x1p20f))) {
             float top = s[0];
 #pragma unroll
-            for (int e = 1; e < 16; ++e) {
+            for (int e = 1; e < 8; ++e) {
                 top = fmaxf(top, s[e]);
             }
-            top               = wave_xor_max(top, 32);
+            top               = wave_xor_max(wave_xor_max(top, 16), 32);
             const float up    = start ? (top == -INFINITY ? 0.0f : top) : fmaxf(top, 0.0f);
             const float alpha = start ? 1.0f : __builtin_amdgcn_exp2f(-up);
             m_ref += up;
@@ -287,32 +323,30 @@ struct WaveRows {
             for (int b = 0; b < kDB; ++b) {
                 o[b] *= alpha;
             }
-            s -= up;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                s[e] -= up;
+            }
             weights();
             start = false;
         }
         l_run += sum;
-        // V^T: lane (d, h), the keys of p: 16 c + 4 h + 0..3 and 16 c + 8 + 4 h + 0..3. A
-        // group of 16 lanes reads eight keys' 16 d and gets them transposed: lane i
-        // points at eight d of key i / 2.
+        pin();
+        // V^T: lane (d, g), the keys of p: 4 g + 0..3 and 16 + 4 g + 0..3. A group of
+        // 16 lanes reads eight keys' 16 d and gets them transposed: ln i points at
+        // eight d of key i / 2.
         typedef int i32x2 __attribute__((ext_vector_type(2)));
         typedef __attribute__((address_space(3))) i32x2* LdsPtr;
-        const int l16 = lane & 15, rr = l16 >> 1;
-        const uint8_t* vp = lv + (4 * h + (rr & 3) + 8 * (rr >> 2)) * T::kPitch +
-                            16 * ((lane >> 4) & 1) + 8 * (l16 & 1);
+        const int rr = (ln & 15) >> 1;
+        const uint8_t* vp = lv + (4 * g + (rr & 3)) * T::kPitch +
+                            (rr >> 2) * (16 * T::kPitch + T::kSkew) + 8 * (ln & 1);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-#pragma unroll
-            for (int b = 0; b < kDB; ++b) {
-                const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                    (LdsPtr)const_cast<uint8_t*>(vp + 16 * c * T::kPitch + 32 * b));
-                const u32x2 x = {static_cast<uint32_t>(w.x), static_cast<uint32_t>(w.y)};
-                o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(e4m3x8_to_bf16x8(x), p[c], o[b], 0, 0, 0);
-                if constexpr (D == 256) {
-                    if (b % 4 == 3) {
-                        pin();
-                    }
-                }
+        for (int b = 0; b < kDB; ++b) {
+            const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((LdsPtr)const_cast<uint8_t*>(vp + 16 * b));
+            const u32x2 x = {static_cast<uint32_t>(w.x), static_cast<uint32_t>(w.y)};
+            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e4m3x8_to_bf16x8(x), p, o[b], 0, 0, 0);
+            if (b % 4 == 3) {
+                pin();
             }
         }
     }
@@ -345,149 +379,137 @@ struct WaveRows {
 #pragma unroll
             for (int u = 0; u < T::kSub; ++u) {
                 const int key0 = i * T::kN + u * kHalf;
-                if (is[u] && key0 < keys.to && key0 + kHalf > keys.from) {
+                if (is[u]) {
                     half(u, keys.from - key0, min(keys.to, end) - key0);
                 }
             }
         }
     }
 
-    // m, l and O of this lane's row to `rows` partials at `part`, row `row`.
-    __device__ __forceinline__ void write(float* part, int64_t rows, int64_t row, bool has) const {
-        const int   h = again(lane) >> 5;
-        const float l = wave_xor_sum(l_run, 32);
-        if (!has) {
-            return;
-        }
-        if (h == 0) {
-            part[row]        = l == 0.0f ? -INFINITY : m_ref;
+    __device__ __forceinline__ static float row_sum(float x) {
+        return wave_xor_sum(wave_xor_sum(x, 16), 32);
+    }
+
+    // m, l (summed over the row's lanes) and O of this lane's row, as one of
+    // `rows` partials at `part`.
+    __device__ __forceinline__ void write(float* part, int64_t rows, int64_t row, float m, float l) const {
+        const int g = lane >> 4;
+        if (g == 0) {
+            part[row]        = m;
             part[rows + row] = l;
         }
-        float* po = part + 2 * rows + row * D + 4 * h;
+        float* po = part + 2 * rows + row * D + 4 * g;
 #pragma unroll
         for (int b = 0; b < kDB; ++b) {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x4 x = {o[b][4 * g], o[b][4 * g + 1], o[b][4 * g + 2], o[b][4 * g + 3]};
-                *reinterpret_cast<f32x4_a4*>(po + 32 * b + 8 * g) = x;
-            }
+            *reinterpret_cast<f32x4_a4*>(po + 16 * b) = o[b];
         }
     }
 
-    // Joins the results of the workgroup's waves into wave 0's, by halves:
-    // the upper half of the waves left hands over (area: what `all` points at).
-    __device__ __forceinline__ void join(float* all, int wave) {
-        l_run = wave_xor_sum(l_run, 32);
-        float mine = l_run == 0.0f ? -INFINITY : m_ref;
+    // Joins the results of the workgroup's waves into wave 0's, by halves: the
+    // upper half of the waves left hands over through LDS. m and l: as write().
+    template <int kW>
+    __device__ __forceinline__ void join(float* all, int wave, float& m, float& l) {
 #pragma unroll
-        for (int n = T::kWaves / 2; n > 0; n >>= 1) {
+        for (int n = kW / 2; n > 0; n >>= 1) {
             __syncthreads();   // tiles, or the step before, are done with
-            // A wave's area: [D / 4 + 1][64 lanes] quads of floats, m and l last.
-            float* a = all + (wave % n) * kHalf * (D + 2);
+            // A wave's area: [D / 16][64 lanes] quads of O, then m and l of 16 rows.
+            float* a = all + (wave % n) * T::kArea;
             if (wave >= n && wave < 2 * n) {
 #pragma unroll
                 for (int b = 0; b < kDB; ++b) {
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const f32x4 x = {o[b][4 * g], o[b][4 * g + 1], o[b][4 * g + 2], o[b][4 * g + 3]};
-                        *reinterpret_cast<f32x4*>(a + ((b * 4 + g) * kWave + lane) * 4) = x;
-                    }
+                    *reinterpret_cast<f32x4*>(a + (b * kWave + lane) * 4) = o[b];
                 }
-                if (lane < 32) {
-                    a[kHalf * D + lane]         = mine;
-                    a[kHalf * D + kHalf + lane] = l_run;
+                if (lane < 16) {
+                    a[16 * D + lane]      = m;
+                    a[16 * D + 16 + lane] = l;
                 }
             }
             __syncthreads();
             if (wave < n) {
-                const float m1 = a[kHalf * D + (lane & 31)], l1 = a[kHalf * D + kHalf + (lane & 31)];
-                float top = fmaxf(mine, m1);
-                if (m1 != m1) {
-                    top = m1;
-                }
-                const float f0 = mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - top);
+                const float m1 = a[16 * D + (lane & 15)], l1 = a[16 * D + 16 + (lane & 15)];
+                const float top = m1 != m1 ? m1 : fmaxf(m, m1);
+                const float f0 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
                 const float f1 = m1 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m1 - top);
-                l_run = f0 * l_run + f1 * l1;
-                mine  = top;
+                l = f0 * l + f1 * l1;
+                m = top;
 #pragma unroll
                 for (int b = 0; b < kDB; ++b) {
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(a + (b * kWave + lane) * 4);
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const f32x4 x = *reinterpret_cast<const f32x4*>(a + ((b * 4 + g) * kWave + lane) * 4);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            o[b][4 * g + i] = f0 * o[b][4 * g + i] + f1 * x[i];
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        o[b][i] = f0 * o[b][i] + f1 * x[i];
                     }
                 }
             }
         }
-        m_ref = mine;
-        l_run *= 0.5f;   // write() adds both halves' lanes
     }
 };
 
 // How a launch is split. Prefix: splits of the keys for each block of rows;
 // own keys: slots of runs.
 struct BatchPlan {
-    int q_blocks;      // blocks of 32 q heads of a kv head
+    int q_blocks;      // blocks of 16 q heads of a kv head
     int slots;
     int splits;        // of the prefix
     int row_blocks;    // of the prefix's rows, of a kv head
     int tile_waves;    // 0: batch_units_kernel takes the prefix, else the waves of batch_prefix_kernel
 };
 
-constexpr int kUnitTiles = 4;   // least tiles of a prefix split of batch_units_kernel
+// Least tiles of a prefix split: a tile for each wave of batch_units_kernel, ...
+constexpr int kUnitTiles = 4;
+#ifndef KT
+#define KT 4
+#endif
+constexpr int kPrefixTiles = KT;
 
-// Workgroups: first (kv head, block of 32 rows, split) of the prefix, then
-// (slot, group of units) of the own keys.
-template <int D>
-__global__ __launch_bounds__(WaveTile<D>::kWaves * kWave, D == 256 ? 1 : 2) void batch_units_kernel(
-    const uint16_t* __restrict__ q, int64_t q_stride, BatchView t, float* __restrict__ own,
-    int* __restrict__ plan, float* __restrict__ shared, BatchPlan bp, int prefix_wgs,
-    float scale_log2) {
+// Workgroup `bid` of the prefix, few rows: (split, block of 16 rows, kv head), the
+// waves taking the split's tiles in turn.
+template <int D, int kW>
+__device__ __forceinline__ void prefix_units(uint8_t* lds, int bid, int prefix,
+                                             const uint16_t* __restrict__ q, int64_t q_stride,
+                                             const BatchView& t, float* __restrict__ shared,
+                                             const BatchPlan& bp, float scale_log2) {
     using T = WaveTile<D>;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
-
     const int tid  = static_cast<int>(threadIdx.x);
-    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-    const int lane = tid & (kWave - 1);
-    const int col  = lane & 31;
+    const int wave = uniform(tid / kWave), lane = tid & (kWave - 1), col = lane & 15;
     const int hq   = t.hkv * t.group;
-    int       bid  = static_cast<int>(blockIdx.x);
-    const int prefix = prefix_keys(t);
-    uint8_t*  mine   = lds + wave * T::kBytes;
-
-    if (bid < prefix_wgs) {
-        const int tiles = (prefix + T::kN - 1) / T::kN;
-        const PrefixRuns runs = prefix_runs(tiles, bp.splits, kUnitTiles);
-        const int at = uniform(bid / t.hkv), kvh = bid - at * t.hkv;
-        const int split = uniform(at / bp.row_blocks), rb = at - split * bp.row_blocks;
-        if (split >= runs.live) {
-            return;
-        }
-        const int rows = t.num_seqs * t.group;
-        const int row  = min(rb * 32 + col, rows - 1);
-        const int b = row / t.group, head = kvh * t.group + (row - b * t.group);
-        WaveRows<D> w(t, mine, lane, kvh, scale_log2);
-        w.load_q(q + b * q_stride + static_cast<int64_t>(head) * D);
-        const int first = split * runs.per;
-        w.run(t.prefix_table, Keys{0, prefix}, first + wave, min(first + runs.per, tiles), T::kWaves,
-              t.lens[b]);
-        w.join(reinterpret_cast<float*>(lds), wave);
-        if (wave == 0) {
-            const int64_t all = static_cast<int64_t>(bp.splits) * t.num_seqs * hq;
-            const int     r2 = rb * 32 + (again(lane) & 31), b2 = r2 / t.group;
-            w.write(shared, all,
-                    (static_cast<int64_t>(split) * t.num_seqs + b2) * hq + kvh * t.group + (r2 - b2 * t.group),
-                    r2 < rows);
-        }
+    const int tiles = (prefix + T::kN - 1) / T::kN;
+    const PrefixRuns runs = prefix_runs(tiles, bp.splits, kUnitTiles);
+    const int at = uniform(bid / t.hkv), kvh = bid - at * t.hkv;
+    const int split = uniform(at / bp.row_blocks), rb = at - split * bp.row_blocks;
+    if (split >= runs.live) {
         return;
     }
-    bid -= prefix_wgs;
+    const int rows = t.num_seqs * t.group;
+    const int row  = min(rb * 16 + col, rows - 1);
+    const int b = row / t.group, head = kvh * t.group + (row - b * t.group);
+    WaveRows<D> w(t, lds + wave * T::kBytes, lane, kvh, scale_log2);
+    w.load_q(q + b * q_stride + static_cast<int64_t>(head) * D);
+    const int first = split * runs.per;
+    w.run(t.prefix_table, Keys{0, prefix}, first + wave, min(first + runs.per, tiles), kW,
+          t.lens[b]);
+    float l = w.row_sum(w.l_run), m = l == 0.0f ? -INFINITY : w.m_ref;
+    w.template join<kW>(reinterpret_cast<float*>(lds), wave, m, l);
+    if (wave == 0 && rb * 16 + col < rows) {
+        const int64_t all = static_cast<int64_t>(bp.splits) * t.num_seqs * hq;
+        w.write(shared, all, (static_cast<int64_t>(split) * t.num_seqs + b) * hq + head, m, l);
+    }
+}
+
+// Workgroup `bid` of the own keys: (slot, group of kW (kv head, block of 16 q heads) units).
+template <int D, int kW>
+__device__ __forceinline__ void own_units(uint8_t* lds, int bid, int prefix,
+                                          const uint16_t* __restrict__ q, int64_t q_stride,
+                                          const BatchView& t, float* __restrict__ own,
+                                          int* __restrict__ plan, const BatchPlan& bp,
+                                          float scale_log2) {
+    using T = WaveTile<D>;
+    const int tid  = static_cast<int>(threadIdx.x);
+    const int wave = uniform(tid / kWave), lane = tid & (kWave - 1), col = lane & 15;
+    const int hq   = t.hkv * t.group;
     const int units  = t.hkv * bp.q_blocks;
-    const int groups = (units + T::kWaves - 1) / T::kWaves;
-    const int slot = uniform(bid / groups), unit = (bid - slot * groups) * T::kWaves + wave;
+    const int groups = (units + kW - 1) / kW;
+    const int slot = uniform(bid / groups), unit = (bid - slot * groups) * kW + wave;
     if (unit >= units) {
         return;
     }
@@ -529,35 +551,47 @@ __global__ __launch_bounds__(WaveTile<D>::kWaves * kWave, D == 256 ? 1 : 2) void
     const Keys keys = own_keys(t, seq, prefix);
     const int t0 = keys.from / T::kN + run * per;
     const int t1 = min(t0 + per, (keys.to - 1) / T::kN + 1);
-    const int head = kvh * t.group + min(qb * 32 + col, t.group - 1);
-    WaveRows<D> w(t, mine, lane, kvh, scale_log2);
+    const int head = kvh * t.group + min(qb * 16 + col, t.group - 1);
+    WaveRows<D> w(t, lds + wave * T::kBytes, lane, kvh, scale_log2);
     w.load_q(q + seq * q_stride + static_cast<int64_t>(head) * D);
     w.run(t.tables + static_cast<int64_t>(seq) * t.table_blocks, keys, t0, t1, 1, keys.to);
-    const int g2 = qb * 32 + (again(lane) & 31);
-    w.write(own, static_cast<int64_t>(bp.slots) * hq, static_cast<int64_t>(slot) * hq + kvh * t.group + g2,
-            g2 < t.group);
+    const float l = w.row_sum(w.l_run);
+    if (qb * 16 + col < t.group) {
+        w.write(own, static_cast<int64_t>(bp.slots) * hq, static_cast<int64_t>(slot) * hq + head,
+                l == 0.0f ? -INFINITY : w.m_ref, l);
+    }
 }
 
 // ---- many rows against the prefix ------------------------------------------------
 
 template <int D, int kW>
-__global__ __launch_bounds__(kW * kWave, D < 256 ? 2 : 1) void batch_prefix_kernel(
-    const uint16_t* __restrict__ q, int64_t q_stride, BatchView t, float* __restrict__ partial,
-    int num_splits, float scale_log2) {
+struct PrefixLds {
+    using T = AttnTile<D>;
+    __attribute__((aligned(16))) uint8_t tiles[T::kBytes];
+    __attribute__((aligned(16))) float   fac[4][2 * T::kN];   // ring of four tiles
+    int                                  here[4][2];          // halves that have a page
+};
+
+// Workgroup `bid` of the prefix: (split, block of 32 kW rows, kv head).
+template <int D, int kW>
+__device__ __forceinline__ void prefix_tiles(PrefixLds<D, kW>& sm, int bid, int prefix,
+                                             const uint16_t* __restrict__ q, int64_t q_stride,
+                                             const BatchView& t, float* __restrict__ partial,
+                                             const BatchPlan& bp, float scale_log2) {
     using T              = AttnTile<D>;
     constexpr int kThr   = kW * kWave;
     constexpr int kCpr   = D / 16;         // 16-code chunks per row
     constexpr int kCopy  = kThr / kCpr;    // rows of one copy step
     constexpr int kSteps = kCopy < T::kN ? T::kN / kCopy : 1;
     constexpr bool kSome = kCopy > T::kN;  // more threads than chunks
-    __shared__ __attribute__((aligned(16))) uint8_t lds[T::kBytes];
-    __shared__ __attribute__((aligned(16))) float   fac[4][2 * T::kN];   // ring of four tiles
-    __shared__ int                                  here[4][2];          // halves that have a page
-
-    const int prefix = prefix_keys(t);
+    uint8_t* const lds = sm.tiles;
+    auto&          fac = sm.fac;
+    auto&          here = sm.here;
+    const int num_splits = bp.splits;
     const int tiles  = (prefix + T::kN - 1) / T::kN;
-    const PrefixRuns runs  = prefix_runs(tiles, num_splits, 1);
-    const int split = static_cast<int>(blockIdx.y);
+    const PrefixRuns runs  = prefix_runs(tiles, num_splits, kPrefixTiles);
+    const int at0   = uniform(bid / t.hkv), hb = bid - at0 * t.hkv;
+    const int split = uniform(at0 / bp.row_blocks), blk = at0 - split * bp.row_blocks;
     if (split >= runs.live) {
         return;
     }
@@ -565,8 +599,6 @@ __global__ __launch_bounds__(kW * kWave, D < 256 ? 2 : 1) void batch_prefix_kern
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int lane = tid & (kWave - 1);
     const int col = lane & 31, h = lane >> 5;
-    const int bid = static_cast<int>(blockIdx.x);
-    const int blk = uniform(bid / t.hkv), hb = bid - blk * t.hkv;
     const int kvh  = uniform((t.hkv & 7) == 0 ? (hb & 7) * (t.hkv >> 3) + (hb >> 3) : hb);
     const int rows = t.num_seqs * t.group;
     const int hq   = t.hkv * t.group;
@@ -746,6 +778,32 @@ __global__ __launch_bounds__(kW * kWave, D < 256 ? 2 : 1) void batch_prefix_kern
     }
 }
 
+// Workgroups: first the prefix's, then those of the own keys. kTiles: the prefix
+// by prefix_tiles, 128 or 256 rows a workgroup, two waves per SIMD (head_dim 256:
+// one); else by prefix_units, three (two).
+template <int D, int kW, bool kTiles>
+__global__ __launch_bounds__(kW * kWave, (D < 256 ? 2 : 1) + (kTiles ? 0 : 1)) void batch_kernel(
+    const uint16_t* __restrict__ q, int64_t q_stride, BatchView t, float* __restrict__ own,
+    int* __restrict__ plan, float* __restrict__ shared, BatchPlan bp, int prefix_wgs,
+    float scale_log2) {
+    union Lds {
+        __attribute__((aligned(16))) uint8_t units[WaveTile<D>::template kLds<kW>];
+        std::conditional_t<kTiles, PrefixLds<D, kW>, int> tiles;
+    };
+    __shared__ Lds lds;
+    const int bid    = static_cast<int>(blockIdx.x);
+    const int prefix = prefix_keys(t);
+    if (bid < prefix_wgs) {
+        if constexpr (kTiles) {
+            prefix_tiles<D, kW>(lds.tiles, bid, prefix, q, q_stride, t, shared, bp, scale_log2);
+        } else {
+            prefix_units<D, kW>(lds.units, bid, prefix, q, q_stride, t, shared, bp, scale_log2);
+        }
+    } else {
+        own_units<D, kW>(lds.units, bid - prefix_wgs, prefix, q, q_stride, t, own, plan, bp, scale_log2);
+    }
+}
+
 // ---- joining a row's partials ------------------------------------------------------
 
 constexpr int kMergeWaves = 4;
@@ -769,7 +827,8 @@ __global__ __launch_bounds__(kMergeWaves * kWave) void batch_merge_kernel(
     const int first = plan[2 * b], n_own = plan[2 * b + 1];
     const int prefix = prefix_keys(t);
     const int n_tile = bp.tile_waves != 0 ? AttnTile<D>::kN : WaveTile<D>::kN;
-    const int n_pre  = prefix_runs((prefix + n_tile - 1) / n_tile, bp.splits, least).live;
+    const int n_pre =
+        prefix > 0 ? prefix_runs((prefix + n_tile - 1) / n_tile, bp.splits, least).live : 0;
     const int64_t own_rows = static_cast<int64_t>(bp.slots) * hq;
     const int64_t pre_rows = static_cast<int64_t>(bp.splits) * t.num_seqs * hq;
     const int n = t.lens[b] > 0 ? n_pre + n_own : 0;
@@ -839,16 +898,24 @@ __global__ __launch_bounds__(kMergeWaves * kWave) void batch_merge_kernel(
     }
 }
 
-BatchPlan batch_plan(int num_seqs, int hq, int hkv, int head_dim, int cus) {
+// `shared`: there is a prefix (its length is known on the device only).
+BatchPlan batch_plan(int num_seqs, int hq, int hkv, int head_dim, int cus, bool shared) {
     const int group = hq / hkv, rows = num_seqs * group;
     BatchPlan p;
-    p.q_blocks   = (group + 31) / 32;
-    p.slots      = num_seqs + std::max(8, 8 * cus / (hkv * p.q_blocks));
-    p.tile_waves = rows <= 128 ? 0 : head_dim < 256 && rows > 128 ? 8 : 4;
-    const int per_block = p.tile_waves == 0 ? 32 : 32 * p.tile_waves;
+    p.q_blocks   = (group + 15) / 16;
+    p.tile_waves = !shared || rows <= 32 ? 0 : head_dim < 256 && rows > 128 ? 8 : 4;
+    const int per_block = p.tile_waves == 0 ? 16 : 32 * p.tile_waves;
     p.row_blocks = (rows + per_block - 1) / per_block;
-    const int wgs = p.row_blocks * hkv;
-    p.splits      = std::max(1, std::min(256, (cus + wgs - 1) / wgs));
+    // Rounds of the chip's workgroups: one for a launch of units (three or, at
+    // head_dim 256, two per compute unit), half of it the prefix's; prefix tiles
+    // take one round of their own.
+    const int waves  = p.tile_waves == 0 ? 4 : p.tile_waves;
+    const int round  = cus * (p.tile_waves == 0 ? (head_dim == 256 ? 2 : 3) : head_dim == 256 ? 1 : 8 / waves);
+    const int wgs    = p.row_blocks * hkv, most = p.tile_waves == 0 ? round / 2 : round;
+    p.splits         = shared ? std::max(1, std::min(256, most / wgs)) : 0;
+    const int left   = shared && p.tile_waves == 0 ? std::max(round - wgs * p.splits, round / 4) : round;
+    const int groups = (hkv * p.q_blocks + waves - 1) / waves;   // workgroups of a slot
+    p.slots = std::max(left / groups, num_seqs + std::max(8, num_seqs / 4));
     return p;
 }
 
@@ -858,28 +925,24 @@ template <int D>
 hipError_t launch_batch(uint16_t* out, int64_t out_stride, const uint16_t* q, int64_t q_stride,
                         const BatchView& t, float* partial, const BatchPlan& p, float scale,
                         hipStream_t stream) {
-    using T                = WaveTile<D>;
     const int   hq         = t.hkv * t.group;
     const float scale_log2 = scale * kLog2e;
     int*        plan       = reinterpret_cast<int*>(partial);
     float*      own        = partial + plan_floats(t.num_seqs);
     float*      shared     = own + static_cast<std::size_t>(p.slots) * hq * (D + 2);
-    const bool  some       = t.prefix_len != nullptr;
-    if (some && p.tile_waves != 0) {
-        const dim3 grid(static_cast<unsigned>(p.row_blocks * t.hkv), static_cast<unsigned>(p.splits));
-        if constexpr (D < 256) {
-            batch_prefix_kernel<D, 8><<<grid, 8 * kWave, 0, stream>>>(q, q_stride, t, shared, p.splits, scale_log2);
-        } else {
-            batch_prefix_kernel<D, 4><<<grid, 4 * kWave, 0, stream>>>(q, q_stride, t, shared, p.splits, scale_log2);
-        }
+    const int   waves      = p.tile_waves == 0 ? 4 : p.tile_waves;
+    const int   pre        = p.row_blocks * t.hkv * p.splits;
+    const dim3  grid(static_cast<unsigned>(pre + p.slots * ((t.hkv * p.q_blocks + waves - 1) / waves)));
+    const dim3  block(static_cast<unsigned>(waves * kWave));
+    if (p.tile_waves == 0) {
+        batch_kernel<D, 4, false><<<grid, block, 0, stream>>>(q, q_stride, t, own, plan, shared, p, pre, scale_log2);
+    } else if (p.tile_waves == 4) {
+        batch_kernel<D, 4, true><<<grid, block, 0, stream>>>(q, q_stride, t, own, plan, shared, p, pre, scale_log2);
+    } else if constexpr (D < 256) {
+        batch_kernel<D, 8, true><<<grid, block, 0, stream>>>(q, q_stride, t, own, plan, shared, p, pre, scale_log2);
     }
-    const int units = t.hkv * p.q_blocks;
-    const int pre   = some && p.tile_waves == 0 ? p.row_blocks * t.hkv * p.splits : 0;
-    const int wgs   = pre + p.slots * ((units + T::kWaves - 1) / T::kWaves);
-    batch_units_kernel<D><<<dim3(static_cast<unsigned>(wgs)), T::kWaves * kWave, 0, stream>>>(
-        q, q_stride, t, own, plan, shared, p, pre, scale_log2);
     const int rows  = t.num_seqs * hq;
-    const int least = p.tile_waves == 0 ? kUnitTiles : 1;
+    const int least = p.tile_waves == 0 ? kUnitTiles : kPrefixTiles;
     if (rows >= 1024) {
         batch_merge_kernel<D, 1><<<dim3(static_cast<unsigned>((rows + kMergeWaves - 1) / kMergeWaves)),
                                    kMergeWaves * kWave, 0, stream>>>(out, out_stride, t, own, plan, shared, p, least);
@@ -894,10 +957,13 @@ hipError_t launch_batch(uint16_t* out, int64_t out_stride, const uint16_t* q, in
 
 std::size_t batch_scratch_floats(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
                                  int cus) {
-    const BatchPlan p = batch_plan(num_seqs, num_q_heads, num_kv_heads, head_dim, cus);
-    return plan_floats(num_seqs) +
-           (static_cast<std::size_t>(p.slots) + static_cast<std::size_t>(p.splits) * num_seqs) *
-               num_q_heads * (head_dim + 2);
+    std::size_t rows = 0;
+    for (const bool shared : {false, true}) {
+        const BatchPlan p = batch_plan(num_seqs, num_q_heads, num_kv_heads, head_dim, cus, shared);
+        rows = std::max(rows, static_cast<std::size_t>(p.slots) +
+                                  static_cast<std::size_t>(p.splits) * num_seqs);
+    }
+    return plan_floats(num_seqs) + rows * num_q_heads * (head_dim + 2);
 }
 
 hipError_t flash_batch_launch(uint16_t* out, int64_t out_stride, const uint16_t* q,
@@ -912,7 +978,8 @@ hipError_t flash_batch_launch(uint16_t* out, int64_t out_stride, const uint16_t*
     if (e != hipSuccess) {
         return e;
     }
-    const BatchPlan p = batch_plan(num_seqs, num_q_heads, num_kv_heads, head_dim, cus);
+    const BatchPlan p =
+        batch_plan(num_seqs, num_q_heads, num_kv_heads, head_dim, cus, prefix_len != nullptr);
     const BatchView t{k, v, k_scale, v_scale, block_tables, table_blocks, lens, prefix_table,
                       prefix_blocks, prefix_len, num_blocks, block_shift, num_seqs,
                       num_q_heads / num_kv_heads, num_kv_heads};
