@@ -116,7 +116,7 @@ def exported_symbols() -> list[str]:
 
 
 def call(name: str, *args) -> None:
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != 0:
         msg = lib.rth_last_error_string().decode()

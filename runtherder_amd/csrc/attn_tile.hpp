@@ -57,6 +57,7 @@ struct QueryRows {
     f32x16 s[2];         // scores of half j in s[j % 2]
     bf16x8 p[2];         // P^T of the half before
     bf16x8 ka[kAhead + 1], va[kAhead + 1];
+    f32x4  fk[4];        // key factors of half j
     float  m_ref, l_run;
     int    lane;
 
@@ -108,12 +109,22 @@ struct QueryRows {
         o[c % kDB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[c & kAhead], p[c / kDB], o[c % kDB], 0, 0, 0);
     }
 
-    // The operand reads that a step starts with.
-    __device__ __forceinline__ void head(const uint8_t* k_at, const uint8_t* v_at) {
+    // The reads that a step starts with: operands, and (kScaled) the key factors kf
+    // of half j.
+    __device__ __forceinline__ void head(const uint8_t* k_at, const uint8_t* v_at,
+                                         const float* kf = nullptr) {
 #pragma unroll
         for (int c = 0; c < kAhead; ++c) {
-            read_k(k_at, c);
             read_v(v_at, c);
+            read_k(k_at, c);
+            if constexpr (kScaled) {
+                if (c == 0) {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        fk[g] = *reinterpret_cast<const f32x4*>(kf + 8 * g + 4 * (lane >> 5));
+                    }
+                }
+            }
         }
     }
 
@@ -127,13 +138,12 @@ struct QueryRows {
     }
 
     // Softmax of half j (in s[kPar], kPar = j % 2), P V of half j - 1 (V rows from v_at),
-    // scores of half j + 1 (K rows from k_at), after head(k_at, v_at).
-    // masked: key r of half j counts as far as r <= lim (lim: less 4 h). kf, vf: the
-    // factors of half j.
+    // scores of half j + 1 (K rows from k_at), after head(k_at, v_at, kf).
+    // masked: key r of half j counts as far as r <= lim (lim: less 4 h). vf: the
+    // value factors of half j.
     template <int kPar>
     __device__ __forceinline__ void step(const uint8_t* k_at, const uint8_t* v_at, float scale_log2,
-                                         const float* kf, const float* vf, bool start, bool masked,
-                                         int lim) {
+                                         const float* vf, bool start, bool masked, int lim) {
         f32x16&   x = s[kPar];
         f32x16&   y = s[kPar ^ 1];
         const int h = lane >> 5;
@@ -142,14 +152,9 @@ struct QueryRows {
         float     sum[2] = {0.0f, 0.0f};
         // Register e of a lane: key 8 (e / 4) + 4 h + e % 4 of the half.
         auto scale4 = [&](int g) {
-            f32x4 f = {scale_log2, scale_log2, scale_log2, scale_log2};
-            if constexpr (kScaled) {
-                f     = *reinterpret_cast<const f32x4*>(kf + 8 * g + 4 * h);
-                fv[g] = *reinterpret_cast<const f32x4*>(vf + 8 * g + 4 * h);
-            }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                x[4 * g + e] = fmaf(x[4 * g + e], f[e], -m_ref);
+                x[4 * g + e] = fmaf(x[4 * g + e], kScaled ? fk[g][e] : scale_log2, -m_ref);
             }
         };
         auto exp4 = [&](int g) {
@@ -164,9 +169,6 @@ struct QueryRows {
                 pn[g >> 1][4 * (g & 1) + e] = static_cast<__bf16>(kScaled ? w[e] * fv[g][e] : w[e]);
             }
         };
-        scale4(0);
-        scale4(1);
-        pin();
         if constexpr (kPrio) {
             __builtin_amdgcn_s_setprio(1);
         }
@@ -176,12 +178,12 @@ struct QueryRows {
             if (c + kAhead < kSteps) {
                 read_v(v_at, c + kAhead);
             }
-            if (c == 0) {
+            if (c == 1) {
                 scale4(2);
                 scale4(3);
             }
             pin();
-            if (c == 0 && masked) {
+            if (c == 1 && masked) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     x[e] = 8 * (e >> 2) + (e & 3) > lim ? -INFINITY : x[e];
@@ -191,9 +193,21 @@ struct QueryRows {
             if (c + kAhead < kSteps) {
                 read_k(k_at, c + kAhead);
             }
+            if (c == 0) {
+                scale4(0);
+                scale4(1);
+            }
+            if constexpr (kScaled) {
+                if (c <= 1) {
+#pragma unroll
+                    for (int g = 2 * c; g < 2 * c + 2; ++g) {
+                        fv[g] = *reinterpret_cast<const f32x4*>(vf + 8 * g + 4 * h);
+                    }
+                }
+            }
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                if (c == 1 + g * (kSteps - 1) / 4 || (kSteps == 4 && c == 3 && 1 + g * 3 / 4 > 3)) {
+                if (c == 2 + g * (kSteps - 2) / 4) {
                     exp4(g);
                 }
             }

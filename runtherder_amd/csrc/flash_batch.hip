@@ -455,12 +455,9 @@ struct BatchPlan {
     int tile_waves;    // 0: batch_units_kernel takes the prefix, else the waves of batch_prefix_kernel
 };
 
-// Least tiles of a prefix split: a tile for each wave of batch_units_kernel, ...
+// Least tiles of a prefix split, by prefix_units (one for each wave) and prefix_tiles.
 constexpr int kUnitTiles = 4;
-#ifndef KT
-#define KT 4
-#endif
-constexpr int kPrefixTiles = KT;
+constexpr int kPrefixTiles = 4;
 
 // Workgroup `bid` of the prefix, few rows: (split, block of 16 rows, kv head), the
 // waves taking the split's tiles in turn.
@@ -569,7 +566,6 @@ struct PrefixLds {
     using T = AttnTile<D>;
     __attribute__((aligned(16))) uint8_t tiles[T::kBytes];
     __attribute__((aligned(16))) float   fac[4][2 * T::kN];   // ring of four tiles
-    int                                  here[4][2];          // halves that have a page
 };
 
 // Workgroup `bid` of the prefix: (split, block of 32 kW rows, kv head).
@@ -586,7 +582,6 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D, kW>& sm, int bid, int 
     constexpr bool kSome = kCopy > T::kN;  // more threads than chunks
     uint8_t* const lds = sm.tiles;
     auto&          fac = sm.fac;
-    auto&          here = sm.here;
     const int num_splits = bp.splits;
     const int tiles  = (prefix + T::kN - 1) / T::kN;
     const PrefixRuns runs  = prefix_runs(tiles, num_splits, kPrefixTiles);
@@ -608,52 +603,67 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D, kW>& sm, int bid, int 
     const int my_seq = my_row / t.group;
     const int tile0 = split * runs.per, n_tiles = min(runs.per, tiles - tile0);
 
-    const int crow = tid / kCpr, cchunk = tid % kCpr;
-    const int64_t stride = static_cast<int64_t>(t.hkv) * D;
-    const int fkey = tid & (T::kN - 1);   // the key whose factor this thread loads (first 2 kN threads)
+    // A thread copies 16 codes of a row in each copy step; the rows of a wave
+    // lie in one half of the tile, so in one page, and their base is scalar.
+    constexpr int kWaveRows = kWave / kCpr;
+    static_assert(kHalf % kWaveRows == 0, "a wave's rows of a copy step lie in one half");
+    const uint32_t stride = static_cast<uint32_t>(t.hkv) * D;
     u32x4 kreg[kSteps], vreg[kSteps];
     float freg = 0.0f;
+    // The pages of a tile's halves, as loaded (in every lane), then as scalars: first
+    // rows, and which halves have a page.
+    struct Entries {
+        int lo, hi;
+    };
     struct Pages {
-        int e[2];
-    };
-    auto entries = [&](int i) {   // of the tile's halves, in every lane
-        Pages p;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int key = (tile0 + i) * T::kN + u * kHalf;
-            p.e[u]        = i < n_tiles && key < prefix ? t.prefix_table[key >> t.block_shift] : -1;
+        int64_t lo, hi;
+        int     there;
+        __device__ __forceinline__ int64_t row(int u) const {
+            const int64_t a = lo, b = hi;
+            return u != 0 ? b : a;
         }
-        return p;
     };
-    // Rows past the prefix, or on no page, are zeros.
-    auto place = [&](int i, const Pages& p, int r, int64_t& row) {
-        const int key  = (tile0 + i) * T::kN + r;
-        const int page = r < kHalf ? p.e[0] : p.e[1];
-        row            = t.row(page, key);
-        return key < prefix && t.is_page(page);
+    auto entries = [&](int i) {
+        const int key = (tile0 + i) * T::kN;
+        auto of = [&](int k) { return i < n_tiles && k < prefix ? t.prefix_table[k >> t.block_shift] : -1; };
+        return Entries{of(key), of(key + kHalf)};
+    };
+    // (A half without a page reads the first one's rows, which nothing uses.)
+    auto pages = [&](int i, const Entries& e) {
+        const int key = (tile0 + i) * T::kN, lo = uniform(e.lo), hi = uniform(e.hi);
+        return Pages{t.row(t.is_page(lo) ? lo : 0, key), t.row(t.is_page(hi) ? hi : 0, key + kHalf),
+                     (t.is_page(lo) ? 1 : 0) | (t.is_page(hi) ? 2 : 0)};
+    };
+    // The row of half u that row r of it reads: past the prefix, its last one.
+    auto row_of = [&](int i, int u, int r) {
+        return static_cast<uint32_t>(min(r, max(prefix - 1 - (tile0 + i) * T::kN - u * kHalf, 0)));
     };
     auto load = [&](const uint8_t* x, int i, const Pages& p, u32x4 (&reg)[kSteps]) {
+        const int tt = again(tid), crow = tt / kCpr, cchunk = tt % kCpr;   // (computed anew: registers)
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            int64_t row;
-            reg[s] = u32x4{};
-            if ((!kSome || crow < T::kN) && place(i, p, s * kCopy + crow, row)) {
-                reg[s] = *reinterpret_cast<const u32x4*>(x + row * stride + static_cast<int64_t>(kvh) * D +
-                                                         16 * cchunk);
+            const int u = kSteps * kCopy / kHalf > 1 || kSome ? (s * kCopy + wave * kWaveRows) / kHalf & 1 : 0;
+            if (!kSome || wave * kWaveRows < T::kN) {
+                const uint8_t* base = x + p.row(u) * stride + static_cast<int64_t>(kvh) * D;
+                const uint32_t off = row_of(i, u, (s * kCopy + crow) & (kHalf - 1)) * stride + 16u * cchunk;
+                reg[s] = *reinterpret_cast<const u32x4*>(base + off);
             }
         }
     };
+    // Factors: of K by the first wave, of V by the second.
     auto load_fac = [&](int i, const Pages& p) {
-        int64_t row;
-        freg = 0.0f;
-        if (tid < 2 * T::kN && place(i, p, fkey, row)) {
-            freg = tid < T::kN ? t.ks[row * t.hkv + kvh] * scale_log2 : t.vs[row * t.hkv + kvh];
+        if (wave < 2) {
+            const int      u = lane >> 5;
+            const float*   x = (wave == 0 ? t.ks : t.vs) + kvh;
+            const int64_t  r = p.row(u) + row_of(i, u, lane & 31);
+            freg = x[r * t.hkv] * (wave == 0 ? scale_log2 : 1.0f);
         }
     };
     auto store = [&](uint32_t to, int pitch, const u32x4 (&reg)[kSteps]) {
+        const int tt = again(tid), crow = tt / kCpr, cchunk = tt % kCpr;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            if (!kSome || crow < T::kN) {
+            if (!kSome || wave * kWaveRows < T::kN) {
                 bf16x8 x, y;
                 e4m3x16_to_bf16x8x2(reg[s], x, y);
                 uint8_t* at = lds + to + (s * kCopy + crow) * pitch + 32 * cchunk;
@@ -662,38 +672,33 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D, kW>& sm, int bid, int 
             }
         }
     };
-    auto store_fac = [&](int i, const Pages& p) {
-        if (tid < 2 * T::kN) {
-            fac[i & 3][tid] = freg;
-        }
-        if (tid < 2) {
-            here[i & 3][tid] = t.is_page(tid == 0 ? p.e[0] : p.e[1]) ? 1 : 0;
+    auto store_fac = [&](int i) {
+        if (wave < 2) {
+            fac[i & 3][wave * T::kN + lane] = freg;
         }
     };
 
-    Pages pk = entries(0);   // of the K tile in kreg (and the factors in freg)
-    Pages pv = pk;           // of the V tile in vreg
-    Pages pn = entries(1);   // of the K tile after it
-    load(t.k, 0, pk, kreg);
-    load_fac(0, pk);
+    // pa, pb: pages of tiles i and i + 1 (at iteration i), e2, e3: entries of the two after.
+    Pages   pa = pages(0, entries(0)), pb = pages(1, entries(1));
+    Entries e2 = entries(2), e3 = entries(3);
+    load(t.k, 0, pa, kreg);
+    load_fac(0, pa);
     const int my_end = min(prefix, t.lens[my_seq]);   // keys this row sees
     QueryRows<D, true, kW == 8> rq;
     rq.lane = lane;
     rq.load_q(q + my_seq * q_stride +
               (static_cast<int64_t>(kvh) * t.group + (my_row - my_seq * t.group)) * D);
-    load(t.v, 0, pv, vreg);
+    load(t.v, 0, pa, vreg);
     rq.clear();
     store(T::k_at(0), T::kKPitch, kreg);
-    store_fac(0, pk);
+    store_fac(0);
     {   // The first step multiplies zero weights with the "tile before".
         const u32x4 zero[kSteps] = {};
         store(T::v_at(1), T::kVPitch, zero);
     }
-    pk = pn;
-    pn = entries(2);
     if (n_tiles > 1) {
-        load(t.k, 1, pk, kreg);
-        load_fac(1, pk);
+        load(t.k, 1, pb, kreg);
+        load_fac(1, pb);
     }
     __syncthreads();
     const int key0 = tile0 * T::kN;
@@ -718,12 +723,11 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D, kW>& sm, int bid, int 
             const int     j    = 2 * i + kPar, at = key0 + 32 * j;
             // (The step past the last half, all of it masked, adds that half's P V.)
             if (j <= mine) {
-                rq.head(lds + k_at, lds + v_at);
-                const bool is  = j < mine && __builtin_amdgcn_readfirstlane(here[i & 3][kPar]) != 0;
+                rq.head(lds + k_at, lds + v_at, fac[i & 3] + kPar * kHalf);
+                const bool is  = j < mine && (pa.there >> kPar & 1) != 0;
                 const int  lim = is ? my_end - 1 - at - 4 * h : -1;
-                rq.template step<kPar>(lds + k_at, lds + v_at, scale_log2, fac[i & 3] + kPar * kHalf,
-                                       fac[i & 3] + T::kN + kPar * kHalf, is && !seen,
-                                       !is || at + 32 > w_end, lim);
+                rq.template step<kPar>(lds + k_at, lds + v_at, scale_log2, fac[i & 3] + T::kN + kPar * kHalf,
+                                       is && !seen, !is || at + 32 > w_end, lim);
                 seen = seen || is;
             }
         };
@@ -731,21 +735,23 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D, kW>& sm, int bid, int 
         // K(i + 1) over K(i - 1), V(i) over V(i - 2): last read before the barrier before.
         if (i + 1 < n_tiles) {
             store(T::k_at(i + 1), T::kKPitch, kreg);
-            store_fac(i + 1, pk);
+            store_fac(i + 1);
         }
         store(T::v_at(i), T::kVPitch, vreg);
         __syncthreads();
-        pv = pk;
-        pk = pn;
-        pn = entries(i + 3);
+        const Pages pc = pages(i + 2, e2);
+        e2 = e3;
+        e3 = entries(i + 4);
         if (i + 2 < n_tiles) {
-            load(t.k, i + 2, pk, kreg);
-            load_fac(i + 2, pk);
+            load(t.k, i + 2, pc, kreg);
+            load_fac(i + 2, pc);
         }
         if (i + 1 < n_tiles) {
-            load(t.v, i + 1, pv, vreg);
+            load(t.v, i + 1, pb, vreg);
         }
         half(std::integral_constant<int, 1>{}, T::k_at(i + 1), T::v_at(i));
+        pa = pb;
+        pb = pc;
     }
     if (idle) {
         return;

@@ -189,7 +189,7 @@ __global__ __launch_bounds__(kW * kWave, D < 256 ? 2 : 1) void flash_packed_kern
             // (The step past the last half, all of it masked, adds that half's P V.)
             if (j <= mine) {
                 rq.head(lds + k_at, lds + v_at);
-                rq.template step<kPar>(lds + k_at, lds + v_at, scale_log2, nullptr, nullptr, j == 0,
+                rq.template step<kPar>(lds + k_at, lds + v_at, scale_log2, nullptr, j == 0,
                                        32 * j + 31 > w_first, my_tok - 32 * j - 4 * h);
             }
         };

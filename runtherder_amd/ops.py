@@ -25,8 +25,21 @@ def _p(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+# The current stream's handle without a torch.cuda.Stream object around it (2.8
+# -> 0.2 us of a call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _current_device() -> int:
+    """The current device; no tensor's where the GPU was never used."""
+    return _get_device() if torch.cuda.is_initialized() else -2
+
+
 def _stream(stream) -> int | None:
     if stream is None:
+        if _raw_stream is not None and torch.cuda.is_initialized():
+            return _raw_stream(_get_device())
         return torch.cuda.current_stream().cuda_stream
     if isinstance(stream, int):
         return stream
@@ -287,38 +300,51 @@ def rmsnorm_lanes(hidden_dim: int) -> int:
 # ---- batches ---------------------------------------------------------------
 # No reference counterparts: the reference serves one sequence at a time.
 
-def _need_rows(t: torch.Tensor, heads: int, head_dim: int, name: str) -> int:
+# The tensors of a call lie on the current device, whose streams it runs on.
+
+def _need_on(t: torch.Tensor, dtype: torch.dtype, name: str, device: int) -> None:
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.get_device() != device:
+        raise TypeError(f"{name} must be a tensor of the current device")
+    if not t.is_contiguous():
+        raise TypeError(f"{name} must be contiguous")
+
+
+def _need_rows(t: torch.Tensor, heads: int, head_dim: int, name: str, device: int) -> int:
     """t: [rows, heads, head_dim] bf16, rows any stride apart; the stride."""
     if t.dtype != torch.bfloat16:
         raise TypeError(f"{name} must be torch.bfloat16, got {t.dtype}")
-    if not t.is_cuda:
-        raise TypeError(f"{name} must be a device tensor")
-    if t.shape[1:] != (heads, head_dim):
-        raise ValueError(f"{name} must be [rows, {heads}, {head_dim}], got {tuple(t.shape)}")
-    s = t.stride()
-    if s[2] != 1 or s[1] != head_dim:
+    if t.get_device() != device:
+        raise TypeError(f"{name} must be a tensor of the current device")
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim:
+        raise ValueError(f"{name} must be [rows, {heads}, {head_dim}], got {tuple(shape)}")
+    if stride[2] != 1 or (stride[1] != head_dim and heads > 1):
         raise TypeError(f"{name}: a row's heads must be contiguous")
-    return s[0] if t.shape[0] > 1 else max(s[0], heads * head_dim)
+    return stride[0] if shape[0] > 1 else max(stride[0], heads * head_dim)
 
 
-def _need_len(t: torch.Tensor, n: int, name: str) -> None:
-    _need(t, torch.int32, name)
+def _need_len(t: torch.Tensor, n: int, name: str, device: int) -> None:
+    _need_on(t, torch.int32, name, device)
     if t.numel() != n:
         raise ValueError(f"{name} must hold {n} ints, got {t.numel()}")
 
 
-def _need_tables(t: torch.Tensor, num_seqs: int, name: str = "block_tables") -> int:
+def _need_tables(t: torch.Tensor, num_seqs: int, name: str, device: int) -> int:
     """t: [num_seqs, table_blocks] int32; table_blocks."""
-    _need(t, torch.int32, name)
-    if t.dim() != 2 or t.shape[0] != num_seqs:
-        raise ValueError(f"{name} must be [{num_seqs}, blocks], got {tuple(t.shape)}")
-    return t.shape[1]
+    _need_on(t, torch.int32, name, device)
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != num_seqs:
+        raise ValueError(f"{name} must be [{num_seqs}, blocks], got {tuple(shape)}")
+    return shape[1]
 
 
-def _need_slabs_of(k, v, k_scale, v_scale, block_size, num_kv_heads, head_dim) -> int:
+def _need_slabs_of(k, v, k_scale, v_scale, block_size, num_kv_heads, head_dim, device) -> int:
     """One layer's paged slabs; the number of blocks."""
-    _need(k, torch.uint8, "k"); _need(v, torch.uint8, "v")
-    _need(k_scale, torch.float32, "k_scale"); _need(v_scale, torch.float32, "v_scale")
+    _need_on(k, torch.uint8, "k", device); _need_on(v, torch.uint8, "v", device)
+    _need_on(k_scale, torch.float32, "k_scale", device)
+    _need_on(v_scale, torch.float32, "v_scale", device)
     rows = k.numel() // (num_kv_heads * head_dim)
     if (block_size < 1 or rows % block_size or k.numel() != rows * num_kv_heads * head_dim
             or v.numel() != k.numel() or k_scale.numel() != rows * num_kv_heads
@@ -334,17 +360,18 @@ def flash_packed_bf16(out, q, k, v, cu_seqlens, num_q_heads, num_kv_heads, head_
     cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of q, out [rows, Hq, D] and k, v
     [rows, Hkv, D] are sequence b. Rows may lie any stride apart (slices of a
     fused projection); rows behind the last sequence stay as they are."""
-    so = _need_rows(out, num_q_heads, head_dim, "out")
-    sq = _need_rows(q, num_q_heads, head_dim, "q")
-    sk = _need_rows(k, num_kv_heads, head_dim, "k")
-    sv = _need_rows(v, num_kv_heads, head_dim, "v")
-    _need(cu_seqlens, torch.int32, "cu_seqlens")
-    n = q.shape[0]
-    if not (out.shape[0] == k.shape[0] == v.shape[0] == n):
+    dev = _current_device()
+    so = _need_rows(out, num_q_heads, head_dim, "out", dev)
+    sq = _need_rows(q, num_q_heads, head_dim, "q", dev)
+    sk = _need_rows(k, num_kv_heads, head_dim, "k", dev)
+    sv = _need_rows(v, num_kv_heads, head_dim, "v", dev)
+    _need_on(cu_seqlens, torch.int32, "cu_seqlens", dev)
+    n = len(q)
+    if not len(out) == len(k) == len(v) == n:
         raise ValueError("out, q, k and v must have the same number of rows")
-    _ffi.call("rth_attn_packed", _p(out), _p(q), _p(k), _p(v), _p(cu_seqlens),
-              cu_seqlens.numel() - 1, n, so, sq, sk, sv, num_q_heads, num_kv_heads, head_dim,
-              float(scale), _stream(stream))
+    _ffi.call("rth_attn_packed", out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+              cu_seqlens.data_ptr(), cu_seqlens.numel() - 1, n, so, sq, sk, sv, num_q_heads,
+              num_kv_heads, head_dim, scale, _stream(stream))
 
 
 def kv_append_fp8_batch(k_cache, v_cache, k_scale, v_scale, k, v, at_pos, block_tables,
@@ -353,21 +380,31 @@ def kv_append_fp8_batch(k_cache, v_cache, k_scale, v_scale, k, v, at_pos, block_
     one row per sequence) to the pages of their sequences, sequence b from
     position at_pos[b] on; bytes as PagedKVCache.append's. Rows without a page
     are not stored."""
-    sk = _need_rows(k, num_kv_heads, head_dim, "k")
-    sv = _need_rows(v, num_kv_heads, head_dim, "v")
-    if k.shape[0] != v.shape[0]:
+    blocks = _need_slabs_of(k_cache, v_cache, k_scale, v_scale, block_size, num_kv_heads,
+                            head_dim, _current_device())
+    _append_batch(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                  k, v, at_pos, block_tables, blocks, block_size, num_kv_heads, head_dim,
+                  cu_seqlens, stream)
+
+
+def _append_batch(kc, vc, ks, vs, k, v, at_pos, block_tables, num_blocks, block_size,
+                  num_kv_heads, head_dim, cu_seqlens, stream):
+    dev = _current_device()
+    sk = _need_rows(k, num_kv_heads, head_dim, "k", dev)
+    sv = _need_rows(v, num_kv_heads, head_dim, "v", dev)
+    n, seqs = len(k), at_pos.numel()
+    if len(v) != n:
         raise ValueError("k and v must have the same number of rows")
-    seqs = at_pos.numel()
-    _need(at_pos, torch.int32, "at_pos")
+    _need_on(at_pos, torch.int32, "at_pos", dev)
     if cu_seqlens is not None:
-        _need_len(cu_seqlens, seqs + 1, "cu_seqlens")
-    elif k.shape[0] != seqs:
+        _need_len(cu_seqlens, seqs + 1, "cu_seqlens", dev)
+        cu_seqlens = cu_seqlens.data_ptr()
+    elif n != seqs:
         raise ValueError("without cu_seqlens, k and v hold one row per sequence")
-    width = _need_tables(block_tables, seqs)
-    blocks = _need_slabs_of(k_cache, v_cache, k_scale, v_scale, block_size, num_kv_heads, head_dim)
-    _ffi.call("rth_kv_append_fp8_batch", _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale), _p(k),
-              _p(v), sk, sv, _p(cu_seqlens), _p(at_pos), seqs, k.shape[0], num_kv_heads, head_dim,
-              _p(block_tables), width, blocks, block_size, _stream(stream))
+    width = _need_tables(block_tables, seqs, "block_tables", dev)
+    _ffi.call("rth_kv_append_fp8_batch", kc, vc, ks, vs, k.data_ptr(), v.data_ptr(), sk, sv,
+              cu_seqlens, at_pos.data_ptr(), seqs, n, num_kv_heads, head_dim,
+              block_tables.data_ptr(), width, num_blocks, block_size, _stream(stream))
 
 
 def batch_scratch_floats(num_seqs: int, num_q_heads: int, num_kv_heads: int,
@@ -384,27 +421,38 @@ def flash_decode_batch_bf16(out, q, k, v, k_scale, v_scale, block_tables, block_
     lie in the pages of prefix_table and are read once for the whole batch; the
     others in block_tables[b], at their own positions. lens[b] <= 0: an unused
     slot, zeros. partial: batch_scratch_floats floats."""
-    so = _need_rows(out, num_q_heads, head_dim, "out")
-    sq = _need_rows(q, num_q_heads, head_dim, "q")
-    seqs = q.shape[0]
-    if out.shape[0] != seqs:
-        raise ValueError("out and q must have the same number of rows")
-    _need_len(lens, seqs, "lens")
-    width = _need_tables(block_tables, seqs)
-    blocks = _need_slabs_of(k, v, k_scale, v_scale, block_size, num_kv_heads, head_dim)
-    _need(partial, torch.float32, "partial")
+    dev, seqs = _current_device(), len(q)
+    blocks = _need_slabs_of(k, v, k_scale, v_scale, block_size, num_kv_heads, head_dim, dev)
+    width = _need_tables(block_tables, seqs, "block_tables", dev)
+    _need_on(partial, torch.float32, "partial", dev)
     if partial.numel() < batch_scratch_floats(seqs, num_q_heads, num_kv_heads, head_dim):
         raise ValueError("partial is smaller than batch_scratch_floats")
-    if (prefix_table is None) != (prefix_len is None):
+    _decode_batch(out, q, k, v, k_scale, v_scale, block_tables, width, blocks, block_size, lens,
+                  partial, num_q_heads, num_kv_heads, head_dim, scale, prefix_table, prefix_len,
+                  stream)
+
+
+def _decode_batch(out, q, k, v, k_scale, v_scale, block_tables, width, num_blocks, block_size,
+                  lens, partial, num_q_heads, num_kv_heads, head_dim, scale, prefix_table,
+                  prefix_len, stream):
+    dev = _current_device()
+    so = _need_rows(out, num_q_heads, head_dim, "out", dev)
+    sq = _need_rows(q, num_q_heads, head_dim, "q", dev)
+    seqs = len(q)
+    if len(out) != seqs:
+        raise ValueError("out and q must have the same number of rows")
+    _need_len(lens, seqs, "lens", dev)
+    pt = pn = pl = 0
+    if prefix_table is not None and prefix_len is not None:
+        _need_on(prefix_table, torch.int32, "prefix_table", dev)
+        _need_len(prefix_len, 1, "prefix_len", dev)
+        pt, pn, pl = prefix_table.data_ptr(), prefix_table.numel(), prefix_len.data_ptr()
+    elif prefix_table is not prefix_len:
         raise ValueError("prefix_table and prefix_len go together")
-    if prefix_table is not None:
-        _need(prefix_table, torch.int32, "prefix_table")
-        _need_len(prefix_len, 1, "prefix_len")
-    _ffi.call("rth_attn_decode_batch", _p(out), so, _p(q), sq, _p(k), _p(v), _p(k_scale),
-              _p(v_scale), _p(block_tables), width, blocks, block_size, _p(lens),
-              _p(prefix_table), 0 if prefix_table is None else prefix_table.numel(),
-              _p(prefix_len), _p(partial), seqs, num_q_heads, num_kv_heads, head_dim,
-              float(scale), _stream(stream))
+    _ffi.call("rth_attn_decode_batch", out.data_ptr(), so, q.data_ptr(), sq, k.data_ptr(),
+              v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(), width,
+              num_blocks, block_size, lens.data_ptr(), pt, pn, pl, partial.data_ptr(), seqs,
+              num_q_heads, num_kv_heads, head_dim, scale, _stream(stream))
 
 
 # ---- interface -------------------------------------------------------------
@@ -448,15 +496,18 @@ class KVSlabs(KVView):
 
 @dataclass(frozen=True)
 class KVBatchView:
-    """One layer of a paged cache with the block tables of a batch
-    (PagedKVCache.batch_view): block_tables [seqs, table_blocks] int32, entries
-    < 0 hold no page. No reference counterpart."""
+    """One layer of a paged cache with the block tables of a batch, as
+    PagedKVCache.batch_view makes it: block_tables [seqs, table_blocks] int32,
+    entries < 0 hold no page. No reference counterpart."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor
     v_scale: torch.Tensor
     block_tables: torch.Tensor
     block_size: int
+    num_blocks: int
+    num_kv_heads: int
+    head_dim: int
 
 
 def _need_slabs(kv):
@@ -577,9 +628,14 @@ class PagedKVCache:
         (cu_seqlens), or one row per sequence, at at_pos[b] of sequence b."""
         if not 0 <= layer < self.num_layers:
             raise ValueError("KVCache append layer out of range")
-        kv_append_fp8_batch(self.k[layer], self.v[layer], self.k_scale[layer],
-                            self.v_scale[layer], k, v, at_pos, block_tables, self.block_size,
-                            self.num_kv_heads, self.head_dim, cu_seqlens, stream)
+        if not self.k.is_cuda:
+            raise TypeError("the cache must be on the device")
+        rows = layer * self.num_blocks * self.block_size * self.num_kv_heads
+        _append_batch(self.k.data_ptr() + rows * self.head_dim,
+                      self.v.data_ptr() + rows * self.head_dim,
+                      self.k_scale.data_ptr() + 4 * rows, self.v_scale.data_ptr() + 4 * rows, k, v,
+                      at_pos, block_tables, self.num_blocks, self.block_size, self.num_kv_heads,
+                      self.head_dim, cu_seqlens, stream)
 
     def batch_view(self, layer, block_tables) -> KVBatchView:
         if not 0 <= layer < self.num_layers:
@@ -588,19 +644,23 @@ class PagedKVCache:
         if block_tables.dim() != 2:
             raise ValueError("block_tables must be [seqs, blocks]")
         return KVBatchView(self.k[layer], self.v[layer], self.k_scale[layer],
-                           self.v_scale[layer], block_tables, self.block_size)
+                           self.v_scale[layer], block_tables, self.block_size, self.num_blocks,
+                           self.num_kv_heads, self.head_dim)
 
     def _all(self):
-        return (_p(self.k), _p(self.v), _p(self.k_scale), _p(self.v_scale), self.num_layers,
-                self.num_blocks, self.block_size, self.num_kv_heads, self.head_dim)
+        return (self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(),
+                self.v_scale.data_ptr(), self.num_layers, self.num_blocks, self.block_size,
+                self.num_kv_heads, self.head_dim)
 
     def copy_pages(self, src, dst, stream=None):
         """Copies page src[i] to page dst[i] in every layer. The dst pages are
         distinct and none of them is a src page."""
-        _need(src, torch.int32, "src")
-        _need_len(dst, src.numel(), "dst")
-        if src.numel():
-            _ffi.call("rth_pages_copy", *self._all(), _p(src), _p(dst), src.numel(),
+        dev = _current_device()
+        _need_on(src, torch.int32, "src", dev)
+        n = src.numel()
+        _need_len(dst, n, "dst", dev)
+        if n:
+            _ffi.call("rth_pages_copy", *self._all(), src.data_ptr(), dst.data_ptr(), n,
                       _stream(stream))
 
 
@@ -638,13 +698,14 @@ class PagePool:
     def reserve(self, block_tables, lens, n_new, stream=None):
         """Pages for positions lens[b] .. lens[b] + n_new[b] - 1 of sequence b,
         where its table row has none yet."""
-        _need(lens, torch.int32, "lens")
-        seqs = lens.numel()
-        _need_len(n_new, seqs, "n_new")
-        width = _need_tables(block_tables, seqs)
-        _ffi.call("rth_pages_reserve", _p(self.refs), _p(self._work), _p(self.status),
-                  self.num_blocks, self.block_size, _p(block_tables), width, _p(lens), _p(n_new),
-                  seqs, _stream(stream))
+        dev, seqs = _current_device(), lens.numel()
+        _need_on(lens, torch.int32, "lens", dev)
+        _need_len(n_new, seqs, "n_new", dev)
+        width = _need_tables(block_tables, seqs, "block_tables", dev)
+        _ffi.call("rth_pages_reserve", self.refs.data_ptr(), self._work.data_ptr(),
+                  self.status.data_ptr(), self.num_blocks, self.block_size,
+                  block_tables.data_ptr(), width, lens.data_ptr(), n_new.data_ptr(), seqs,
+                  _stream(stream))
 
     def fork(self, cache, dst_tables, dst_lens, src_tables, src_lens, parents, stream=None):
         """Sequence i of dst becomes a copy of sequence parents[i] of src (any
@@ -653,37 +714,39 @@ class PagePool:
         layers of `cache`, into a page of the child's own. The dst tables hold no
         pages before (free them first)."""
         self._of(cache)
-        _need(parents, torch.int32, "parents"); _need(src_lens, torch.int32, "src_lens")
-        n = parents.numel()
-        _need_len(dst_lens, n, "dst_lens")
-        width = _need_tables(src_tables, src_lens.numel(), "src_tables")
-        if _need_tables(dst_tables, n, "dst_tables") != width:
+        dev, n, seqs = _current_device(), parents.numel(), src_lens.numel()
+        _need_on(parents, torch.int32, "parents", dev)
+        _need_on(src_lens, torch.int32, "src_lens", dev)
+        _need_len(dst_lens, n, "dst_lens", dev)
+        width = _need_tables(src_tables, seqs, "src_tables", dev)
+        if _need_tables(dst_tables, n, "dst_tables", dev) != width:
             raise ValueError("dst_tables and src_tables must have the same number of blocks")
-        _ffi.call("rth_pages_fork", *cache._all(), _p(self.refs), _p(self._work), _p(self.status),
-                  _p(dst_tables), _p(dst_lens), _p(src_tables), _p(src_lens), width,
-                  src_lens.numel(), _p(parents), n, _stream(stream))
+        _ffi.call("rth_pages_fork", *cache._all(), self.refs.data_ptr(), self._work.data_ptr(),
+                  self.status.data_ptr(), dst_tables.data_ptr(), dst_lens.data_ptr(),
+                  src_tables.data_ptr(), src_lens.data_ptr(), width, seqs, parents.data_ptr(), n,
+                  _stream(stream))
 
     def free(self, block_tables, lens, drop=None, stream=None):
         """Frees the sequences with drop[b] != 0 (None: all): their pages lose
         one reference, their table rows hold none, their lengths are 0."""
-        _need(lens, torch.int32, "lens")
-        seqs = lens.numel()
-        width = _need_tables(block_tables, seqs)
+        dev, seqs = _current_device(), lens.numel()
+        _need_on(lens, torch.int32, "lens", dev)
+        width = _need_tables(block_tables, seqs, "block_tables", dev)
         if drop is not None:
-            _need_len(drop, seqs, "drop")
-        _ffi.call("rth_pages_free", _p(self.refs), self.num_blocks, _p(block_tables), width,
-                  _p(lens), _p(drop), seqs, _stream(stream))
+            _need_len(drop, seqs, "drop", dev)
+            drop = drop.data_ptr()
+        _ffi.call("rth_pages_free", self.refs.data_ptr(), self.num_blocks,
+                  block_tables.data_ptr(), width, lens.data_ptr(), drop, seqs, _stream(stream))
 
     def compact(self, cache, block_tables, stream=None):
         """Moves the pages in use down to the lowest ones, in all layers of
         `cache`, and renames them in block_tables, which are all the tables that
         hold pages of the pool."""
         self._of(cache)
-        if block_tables.dim() != 2:
-            raise ValueError("block_tables must be [seqs, blocks]")
-        width = _need_tables(block_tables, block_tables.shape[0])
-        _ffi.call("rth_pages_compact", *cache._all(), _p(self.refs), _p(self._work),
-                  _p(block_tables), width, block_tables.shape[0], _stream(stream))
+        seqs = len(block_tables)
+        width = _need_tables(block_tables, seqs, "block_tables", _current_device())
+        _ffi.call("rth_pages_compact", *cache._all(), self.refs.data_ptr(),
+                  self._work.data_ptr(), block_tables.data_ptr(), width, seqs, _stream(stream))
 
 
 class AttentionBackend:
@@ -856,12 +919,17 @@ class BatchAttention:
     def run_decode(self, out, q, kv: KVBatchView, lens, prefix_table=None, prefix_len=None,
                    stream=None):
         """flash_decode_batch_bf16 over kv with this object's scratch."""
-        c = self.config
-        if q.shape[0] > self.max_seqs:
-            raise ValueError(f"{q.shape[0]} sequences: this backend was made for {self.max_seqs}")
-        flash_decode_batch_bf16(out, q, kv.k, kv.v, kv.k_scale, kv.v_scale, kv.block_tables,
-                                kv.block_size, lens, self.partial, c.num_q_heads, c.num_kv_heads,
-                                c.head_dim, c.scale, prefix_table, prefix_len, stream)
+        c, tables = self.config, kv.block_tables
+        seqs, width = tables.shape
+        if len(q) != seqs:
+            raise ValueError(f"q holds {len(q)} sequences, the view {seqs}")
+        if seqs > self.max_seqs:
+            raise ValueError(f"{seqs} sequences: this backend was made for {self.max_seqs}")
+        if kv.num_kv_heads != c.num_kv_heads or kv.head_dim != c.head_dim:
+            raise ValueError("the view and the configuration differ in their kv heads")
+        _decode_batch(out, q, kv.k, kv.v, kv.k_scale, kv.v_scale, tables, width, kv.num_blocks,
+                      kv.block_size, lens, self.partial, c.num_q_heads, c.num_kv_heads, c.head_dim,
+                      c.scale, prefix_table, prefix_len, stream)
 
 
 class NaiveAttention(AttentionBackend):
