@@ -27,32 +27,40 @@ struct AppendSlab {
     int64_t         stride;   // elements per token
 };
 
-template <int kLanes>   // lanes per row, 8 elements each
+// kLanes lanes per row, kChunks chunks of 8 elements each (chunk sub + c * kLanes).
+template <int kLanes, int kChunks>
 __global__ __launch_bounds__(kAppendBlock) void append_batch_kernel(
     AppendSlab s0, AppendSlab s1, const int* __restrict__ cu, const int* __restrict__ at_pos,
     int num_seqs, int num_rows, int hkv, int head_dim, const int* __restrict__ tables,
     int table_blocks, int num_blocks, int block_shift) {
-    constexpr int    kRows = kWave / kLanes;   // of a wave
-    const AppendSlab s     = blockIdx.y == 0 ? s0 : s1;
-    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-    const int sub = lane % kLanes, mine = lane / kLanes;
-    const int64_t row0 = (static_cast<int64_t>(blockIdx.x) * kAppendBlock + threadIdx.x - lane) / kLanes;
-    const int64_t row  = row0 + mine;
-    const int64_t end  = static_cast<int64_t>(num_rows) * hkv;
-    const bool    has  = row < end && 8 * sub < head_dim;
-    const int     tok  = static_cast<int>(row / hkv), kvh = static_cast<int>(row % hkv);
+    constexpr uint32_t kRows = kWave / kLanes;   // of a wave
+    const AppendSlab s    = blockIdx.y == 0 ? s0 : s1;
+    const int        lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    const int        sub = lane % kLanes, mine = lane / kLanes;
+    const uint32_t   heads = static_cast<uint32_t>(hkv);
+    const uint32_t   end   = static_cast<uint32_t>(num_rows) * heads;   // below 2^31
+    const uint32_t   row0  = static_cast<uint32_t>(
+        uniform(static_cast<int>((blockIdx.x * kAppendBlock + (threadIdx.x & ~(kWave - 1u))) / kLanes)));
+    const uint32_t row = row0 + mine;
+    const bool     has = row < end;
+    const int      tok = static_cast<int>(row / heads), kvh = static_cast<int>(row - tok * heads);
 
-    u32x4 x = {};
-    if (has) {
-        x = *reinterpret_cast<const u32x4*>(s.x + tok * s.stride + static_cast<int64_t>(kvh) * head_dim +
-                                            8 * sub);
+    u32x4           x[kChunks];
+    const uint16_t* from = s.x + tok * s.stride + static_cast<int64_t>(kvh) * head_dim;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        const int e = 8 * (sub + c * kLanes);
+        x[c]        = u32x4{};
+        if (has && e < head_dim) {
+            x[c] = *reinterpret_cast<const u32x4*>(from + e);
+        }
     }
     // The sequence of each of the wave's tokens.
     int seq = tok;
     if (cu != nullptr) {
         seq = 0;
-        const int first = static_cast<int>(row0 / hkv);
-        const int last  = static_cast<int>((min(row0 + kRows, end) - 1) / hkv);
+        const int first = static_cast<int>(row0 / heads);
+        const int last  = static_cast<int>((min(row0 + kRows, end) - 1) / heads);
         for (int b0 = 0; b0 < num_seqs; b0 += kWave) {
             const int b   = b0 + lane;
             const int top = b < num_seqs ? cu[b + 1] : INT32_MAX;
@@ -64,8 +72,9 @@ __global__ __launch_bounds__(kAppendBlock) void append_batch_kernel(
     }
     int64_t dst = -1;
     if (has && seq < num_seqs) {
-        const int64_t p = static_cast<int64_t>(at_pos[seq]) + (cu != nullptr ? tok - cu[seq] : 0);
-        if (p >= 0 && (p >> block_shift) < table_blocks && (cu == nullptr || tok >= cu[seq])) {
+        const int     begin = cu != nullptr ? cu[seq] : tok;
+        const int64_t p     = static_cast<int64_t>(at_pos[seq]) + tok - begin;
+        if (tok >= begin && p >= 0 && (p >> block_shift) < table_blocks) {
             const int page = tables[static_cast<int64_t>(seq) * table_blocks + (p >> block_shift)];
             if (page >= 0 && page < num_blocks) {
                 const int64_t at = (static_cast<int64_t>(page) << block_shift) +
@@ -77,9 +86,12 @@ __global__ __launch_bounds__(kAppendBlock) void append_batch_kernel(
 
     float amax = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        amax = fmaxf(amax, fabsf(__uint_as_float(x[e] << 16)));
-        amax = fmaxf(amax, fabsf(__uint_as_float(x[e] & 0xffff0000u)));
+    for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            amax = fmaxf(amax, fabsf(__uint_as_float(x[c][e] << 16)));
+            amax = fmaxf(amax, fabsf(__uint_as_float(x[c][e] & 0xffff0000u)));
+        }
     }
 #pragma unroll
     for (int m = 1; m < kLanes; m <<= 1) {
@@ -92,12 +104,19 @@ __global__ __launch_bounds__(kAppendBlock) void append_batch_kernel(
     if (sub == 0) {
         s.scale[dst] = amax / kE4M3Max;
     }
-    uint32_t lo = 0, hi = 0;
-    lo = e4m3x2_pack<false>(__uint_as_float(x.x << 16) * inv, __uint_as_float(x.x & 0xffff0000u) * inv, lo);
-    lo = e4m3x2_pack<true>(__uint_as_float(x.y << 16) * inv, __uint_as_float(x.y & 0xffff0000u) * inv, lo);
-    hi = e4m3x2_pack<false>(__uint_as_float(x.z << 16) * inv, __uint_as_float(x.z & 0xffff0000u) * inv, hi);
-    hi = e4m3x2_pack<true>(__uint_as_float(x.w << 16) * inv, __uint_as_float(x.w & 0xffff0000u) * inv, hi);
-    *reinterpret_cast<u32x2*>(s.q + dst * head_dim + 8 * sub) = u32x2{lo, hi};
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        const int e = 8 * (sub + c * kLanes);
+        auto      f = [&](uint32_t w, bool hi) { return __uint_as_float(hi ? w & 0xffff0000u : w << 16) * inv; };
+        uint32_t  lo = 0, hi = 0;
+        lo = e4m3x2_pack<false>(f(x[c].x, false), f(x[c].x, true), lo);
+        lo = e4m3x2_pack<true>(f(x[c].y, false), f(x[c].y, true), lo);
+        hi = e4m3x2_pack<false>(f(x[c].z, false), f(x[c].z, true), hi);
+        hi = e4m3x2_pack<true>(f(x[c].w, false), f(x[c].w, true), hi);
+        if (e < head_dim) {
+            *reinterpret_cast<u32x2*>(s.q + dst * head_dim + e) = u32x2{lo, hi};
+        }
+    }
 }
 
 }  // namespace
@@ -112,28 +131,46 @@ hipError_t kv_append_batch_launch(uint8_t* k_q, uint8_t* v_q, float* k_scale, fl
     while (8 * lanes < head_dim) {
         lanes <<= 1;
     }
-    const int64_t rows = static_cast<int64_t>(num_rows) * num_kv_heads;
-    const int64_t per  = kAppendBlock / lanes;
+    // Large appends: half the lanes per row, so that each has two loads in flight and a
+    // wave's search of the sequences serves twice the rows; small ones finish
+    // sooner with the wider groups.
+    const int64_t rows  = static_cast<int64_t>(num_rows) * num_kv_heads;
+    const bool    large = 2 * rows >= 32768 && lanes >= 8;
+    lanes               = large ? lanes / 2 : lanes;
+    const int64_t per   = kAppendBlock / lanes;
     const dim3    grid(static_cast<unsigned>((rows + per - 1) / per), 2);
     const AppendSlab sk{k_q, k_scale, k, k_stride}, sv{v_q, v_scale, v, v_stride};
-    switch (lanes) {
-#define RTH_CASE(L)                                                                            \
-    case L:                                                                                    \
-        append_batch_kernel<L><<<grid, kAppendBlock, 0, stream>>>(                             \
-            sk, sv, cu_seqlens, at_pos, num_seqs, num_rows, num_kv_heads, head_dim, block_tables, \
-            table_blocks, num_blocks, block_shift);                                            \
+#define RTH_APPEND(L, C)                                                                          \
+    append_batch_kernel<L, C><<<grid, kAppendBlock, 0, stream>>>(                                 \
+        sk, sv, cu_seqlens, at_pos, num_seqs, num_rows, num_kv_heads, head_dim, block_tables,     \
+        table_blocks, num_blocks, block_shift)
+#define RTH_CASE(L)            \
+    case L:                    \
+        if (large) {           \
+            RTH_APPEND(L, 2);  \
+        } else {               \
+            RTH_APPEND(L, 1);  \
+        }                      \
         break;
-        RTH_CASE(1)
-        RTH_CASE(2)
+    switch (lanes) {
+        case 1:
+            RTH_APPEND(1, 1);
+            break;
+        case 2:
+            RTH_APPEND(2, 1);
+            break;
         RTH_CASE(4)
         RTH_CASE(8)
         RTH_CASE(16)
         RTH_CASE(32)
-        RTH_CASE(64)
-#undef RTH_CASE
+        case 64:
+            RTH_APPEND(64, 1);
+            break;
         default:
             return hipErrorInvalidValue;
     }
+#undef RTH_CASE
+#undef RTH_APPEND
     return hipGetLastError();
 }
 
