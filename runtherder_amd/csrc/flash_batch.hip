@@ -450,14 +450,12 @@ struct WaveRows {
 struct BatchPlan {
     int q_blocks;      // blocks of 16 q heads of a kv head
     int slots;
+    int waves;         // of a workgroup
     int splits;        // of the prefix
     int row_blocks;    // of the prefix's rows, of a kv head
-    int tile_waves;    // 0: batch_units_kernel takes the prefix, else the waves of batch_prefix_kernel
+    int least;         // tiles of a split, if there are as many
+    int tile_waves;    // 0: prefix_units takes the prefix; else the waves of a block of prefix_tiles's rows
 };
-
-// Least tiles of a prefix split, by prefix_units (one for each wave) and prefix_tiles.
-constexpr int kUnitTiles = 4;
-constexpr int kPrefixTiles = 4;
 
 // Workgroup `bid` of the prefix, few rows: (split, block of 16 rows, kv head), the
 // waves taking the split's tiles in turn.
@@ -471,7 +469,7 @@ __device__ __forceinline__ void prefix_units(uint8_t* lds, int bid, int prefix,
     const int wave = uniform(tid / kWave), lane = tid & (kWave - 1), col = lane & 15;
     const int hq   = t.hkv * t.group;
     const int tiles = (prefix + T::kN - 1) / T::kN;
-    const PrefixRuns runs = prefix_runs(tiles, bp.splits, kUnitTiles);
+    const PrefixRuns runs = prefix_runs(tiles, bp.splits, bp.least);
     const int at = uniform(bid / t.hkv), kvh = bid - at * t.hkv;
     const int split = uniform(at / bp.row_blocks), rb = at - split * bp.row_blocks;
     if (split >= runs.live) {
@@ -561,38 +559,42 @@ __device__ __forceinline__ void own_units(uint8_t* lds, int bid, int prefix,
 
 // ---- many rows against the prefix ------------------------------------------------
 
-template <int D, int kW>
+template <int D>
 struct PrefixLds {
     using T = AttnTile<D>;
     __attribute__((aligned(16))) uint8_t tiles[T::kBytes];
     __attribute__((aligned(16))) float   fac[4][2 * T::kN];   // ring of four tiles
 };
 
-// Workgroup `bid` of the prefix: (split, block of 32 kW rows, kv head).
-template <int D, int kW>
-__device__ __forceinline__ void prefix_tiles(PrefixLds<D, kW>& sm, int bid, int prefix,
+// Workgroup `bid` of the prefix: (split, block of 32 kW rows, kv head). kG groups of
+// kW waves share its tiles, each with a part of the split of its own, and join
+// their results in LDS: a split of few rows is done in half the time, and its partial is
+// written once.
+template <int D, int kW, int kG>
+__device__ __forceinline__ void prefix_tiles(PrefixLds<D> (&sm)[kG], int bid, int prefix,
                                              const uint16_t* __restrict__ q, int64_t q_stride,
                                              const BatchView& t, float* __restrict__ partial,
                                              const BatchPlan& bp, float scale_log2) {
     using T              = AttnTile<D>;
-    constexpr int kThr   = kW * kWave;
+    constexpr int kThr   = kW * kWave;     // of a group
     constexpr int kCpr   = D / 16;         // 16-code chunks per row
     constexpr int kCopy  = kThr / kCpr;    // rows of one copy step
     constexpr int kSteps = kCopy < T::kN ? T::kN / kCopy : 1;
     constexpr bool kSome = kCopy > T::kN;  // more threads than chunks
-    uint8_t* const lds = sm.tiles;
-    auto&          fac = sm.fac;
     const int num_splits = bp.splits;
     const int tiles  = (prefix + T::kN - 1) / T::kN;
-    const PrefixRuns runs  = prefix_runs(tiles, num_splits, kPrefixTiles);
+    const PrefixRuns runs  = prefix_runs(tiles, num_splits, bp.least);
     const int at0   = uniform(bid / t.hkv), hb = bid - at0 * t.hkv;
     const int split = uniform(at0 / bp.row_blocks), blk = at0 - split * bp.row_blocks;
     if (split >= runs.live) {
         return;
     }
-    const int tid  = static_cast<int>(threadIdx.x);
-    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int group = kG == 1 ? 0 : uniform(static_cast<int>(threadIdx.x) / kThr);
+    const int tid   = static_cast<int>(threadIdx.x) - group * kThr;
+    const int wave = uniform(tid / kWave);
     const int lane = tid & (kWave - 1);
+    uint8_t* const lds = sm[group].tiles;
+    auto&          fac = sm[group].fac;
     const int col = lane & 31, h = lane >> 5;
     const int kvh  = uniform((t.hkv & 7) == 0 ? (hb & 7) * (t.hkv >> 3) + (hb >> 3) : hb);
     const int rows = t.num_seqs * t.group;
@@ -601,7 +603,11 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D, kW>& sm, int bid, int 
     const bool idle = wr0 >= rows;
     const int my_row = min(wr0 + col, rows - 1);
     const int my_seq = my_row / t.group;
-    const int tile0 = split * runs.per, n_tiles = min(runs.per, tiles - tile0);
+    // The split's tiles, and this group's of them (rounds: the first group's).
+    const int all_tiles = min(runs.per, tiles - split * runs.per);
+    const int rounds    = (all_tiles + kG - 1) / kG;
+    const int tile0     = split * runs.per + group * rounds;
+    const int n_tiles   = min(rounds, all_tiles - group * rounds);
 
     // A thread copies 16 codes of a row in each copy step; the rows of a wave
     // lie in one half of the tile, so in one page, and their base is scalar.
@@ -681,17 +687,21 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D, kW>& sm, int bid, int 
     // pa, pb: pages of tiles i and i + 1 (at iteration i), e2, e3: entries of the two after.
     Pages   pa = pages(0, entries(0)), pb = pages(1, entries(1));
     Entries e2 = entries(2), e3 = entries(3);
-    load(t.k, 0, pa, kreg);
-    load_fac(0, pa);
+    if (n_tiles > 0) {
+        load(t.k, 0, pa, kreg);
+        load_fac(0, pa);
+    }
     const int my_end = min(prefix, t.lens[my_seq]);   // keys this row sees
     QueryRows<D, true, kW == 8> rq;
     rq.lane = lane;
     rq.load_q(q + my_seq * q_stride +
               (static_cast<int64_t>(kvh) * t.group + (my_row - my_seq * t.group)) * D);
-    load(t.v, 0, pa, vreg);
+    if (n_tiles > 0) {
+        load(t.v, 0, pa, vreg);
+        store(T::k_at(0), T::kKPitch, kreg);
+        store_fac(0);
+    }
     rq.clear();
-    store(T::k_at(0), T::kKPitch, kreg);
-    store_fac(0);
     {   // The first step multiplies zero weights with the "tile before".
         const u32x4 zero[kSteps] = {};
         store(T::v_at(1), T::kVPitch, zero);
@@ -703,7 +713,7 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D, kW>& sm, int bid, int 
     __syncthreads();
     const int key0 = tile0 * T::kN;
     // Halves with keys; a half that reaches past w_end is masked.
-    const int mine = idle ? -1 : (min(prefix - key0, n_tiles * T::kN) + kHalf - 1) / kHalf;
+    const int mine = idle || n_tiles <= 0 ? -1 : (min(prefix - key0, n_tiles * T::kN) + kHalf - 1) / kHalf;
     int       w_end;
     {
         int m = my_end;
@@ -717,7 +727,7 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D, kW>& sm, int bid, int 
     if (mine > 0) {
         rq.first_scores(lds + T::k_at(0));
     }
-    for (int i = 0; i < n_tiles; ++i) {
+    for (int i = 0; i < rounds; ++i) {
         auto half = [&](auto par, uint32_t k_at, uint32_t v_at) {
             constexpr int kPar = decltype(par)::value;
             const int     j    = 2 * i + kPar, at = key0 + 32 * j;
@@ -737,7 +747,9 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D, kW>& sm, int bid, int 
             store(T::k_at(i + 1), T::kKPitch, kreg);
             store_fac(i + 1);
         }
-        store(T::v_at(i), T::kVPitch, vreg);
+        if (i < n_tiles) {
+            store(T::v_at(i), T::kVPitch, vreg);
+        }
         __syncthreads();
         const Pages pc = pages(i + 2, e2);
         e2 = e3;
@@ -753,22 +765,64 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D, kW>& sm, int bid, int 
         pa = pb;
         pb = pc;
     }
+    if (mine == 2 * rounds) {
+        rq.last(lds + T::v_at(rounds - 1) + 32 * T::kVPitch);
+    }
+    float l = wave_xor_sum(rq.l_run, 32);
+    float m = l == 0.0f ? -INFINITY : rq.m_ref;
+    if constexpr (kG == 2) {
+        // The second group hands over: [D / 8][64 lanes] quads of O, then m and l.
+        float* area = reinterpret_cast<float*>(sm) + wave * 32 * (D + 2);
+        static_assert(kW * 32 * (D + 2) * 4 <= static_cast<int>(sizeof(sm)), "");
+        __syncthreads();
+        if (group == 1) {
+#pragma unroll
+            for (int b = 0; b < D / 32; ++b) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 x = {rq.o[b][4 * g], rq.o[b][4 * g + 1], rq.o[b][4 * g + 2], rq.o[b][4 * g + 3]};
+                    *reinterpret_cast<f32x4*>(area + ((b * 4 + g) * kWave + lane) * 4) = x;
+                }
+            }
+            if (h == 0) {
+                area[32 * D + col]      = m;
+                area[32 * D + 32 + col] = l;
+            }
+        }
+        __syncthreads();
+        if (group == 1) {
+            return;
+        }
+        const float m1 = area[32 * D + col], l1 = area[32 * D + 32 + col];
+        const float top = m1 != m1 ? m1 : fmaxf(m, m1);
+        const float f0 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+        const float f1 = m1 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m1 - top);
+        m = top;
+        l = f0 * l + f1 * l1;
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(area + ((b * 4 + g) * kWave + lane) * 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    rq.o[b][4 * g + i] = f0 * rq.o[b][4 * g + i] + f1 * x[i];
+                }
+            }
+        }
+    }
     if (idle) {
         return;
     }
-    if (mine == 2 * n_tiles) {
-        rq.last(lds + T::v_at(n_tiles - 1) + 32 * T::kVPitch);
-    }
     // Partials: [splits, B, Hq] m, l, then O.
     const int64_t all = static_cast<int64_t>(num_splits) * t.num_seqs * hq;
-    const float   l   = wave_xor_sum(rq.l_run, 32);
     const int     ln = again(lane), r = uniform(wr0) + (ln & 31), h2 = ln >> 5;
     if (r < rows) {
         const int     b   = r / again(t.group);
         const int     g   = r - b * t.group;
         const int64_t row = (static_cast<int64_t>(split) * t.num_seqs + b) * hq + kvh * t.group + g;
         if (h2 == 0) {
-            partial[row]       = l == 0.0f ? -INFINITY : rq.m_ref;
+            partial[row]       = m;
             partial[all + row] = l;
         }
         float* po = partial + 2 * all + row * D + 4 * h2;
@@ -784,29 +838,32 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D, kW>& sm, int bid, int 
     }
 }
 
-// Workgroups: first the prefix's, then those of the own keys. kTiles: the prefix
-// by prefix_tiles, 128 or 256 rows a workgroup, two waves per SIMD (head_dim 256:
-// one); else by prefix_units, three (two).
-template <int D, int kW, bool kTiles>
-__global__ __launch_bounds__(kW * kWave, (D < 256 ? 2 : 1) + (kTiles ? 0 : 1)) void batch_kernel(
+// Workgroups: first the prefix's, then those of the own keys. kG > 0: the prefix by
+// prefix_tiles, two waves per SIMD (head_dim 256: one); kG == 0: by prefix_units,
+// three (two).
+constexpr int batch_waves(int w, int g) { return w * (g > 0 ? g : 1); }
+template <int D, int kW, int kG>
+__global__ __launch_bounds__(batch_waves(kW, kG) * kWave, (D < 256 ? 2 : 1) + (kG > 0 ? 0 : 1)) void batch_kernel(
     const uint16_t* __restrict__ q, int64_t q_stride, BatchView t, float* __restrict__ own,
     int* __restrict__ plan, float* __restrict__ shared, BatchPlan bp, int prefix_wgs,
     float scale_log2) {
+    constexpr int kWaves = batch_waves(kW, kG);
     union Lds {
-        __attribute__((aligned(16))) uint8_t units[WaveTile<D>::template kLds<kW>];
-        std::conditional_t<kTiles, PrefixLds<D, kW>, int> tiles;
+        __attribute__((aligned(16))) uint8_t units[WaveTile<D>::template kLds<kWaves>];
+        PrefixLds<D> tiles[kG > 0 ? kG : 1];
     };
-    __shared__ Lds lds;
+    __shared__ std::conditional_t<(kG > 0), Lds, uint8_t[WaveTile<D>::template kLds<kWaves>]> lds;
+    uint8_t*  units  = reinterpret_cast<uint8_t*>(&lds);
     const int bid    = static_cast<int>(blockIdx.x);
     const int prefix = prefix_keys(t);
     if (bid < prefix_wgs) {
-        if constexpr (kTiles) {
-            prefix_tiles<D, kW>(lds.tiles, bid, prefix, q, q_stride, t, shared, bp, scale_log2);
+        if constexpr (kG > 0) {
+            prefix_tiles<D, kW, kG>(lds.tiles, bid, prefix, q, q_stride, t, shared, bp, scale_log2);
         } else {
-            prefix_units<D, kW>(lds.units, bid, prefix, q, q_stride, t, shared, bp, scale_log2);
+            prefix_units<D, kWaves>(units, bid, prefix, q, q_stride, t, shared, bp, scale_log2);
         }
     } else {
-        own_units<D, kW>(lds.units, bid - prefix_wgs, prefix, q, q_stride, t, own, plan, bp, scale_log2);
+        own_units<D, kWaves>(units, bid - prefix_wgs, prefix, q, q_stride, t, own, plan, bp, scale_log2);
     }
 }
 
@@ -814,94 +871,97 @@ __global__ __launch_bounds__(kW * kWave, (D < 256 ? 2 : 1) + (kTiles ? 0 : 1)) v
 
 constexpr int kMergeWaves = 4;
 
-// kRow: waves per row (1: a row per wave, for many rows). A group of D / 4
-// lanes takes every (groups)-th partial, four floats a lane.
-template <int D, int kRow>
+// A workgroup joins the partials of a row: each group of D / 4 lanes (four floats a
+// lane) every kGroups-th one against a maximum of its own, four on the way
+// at a time, so that nothing waits for the maximum of all; then the groups.
+template <int D>
 __global__ __launch_bounds__(kMergeWaves * kWave) void batch_merge_kernel(
     uint16_t* __restrict__ out, int64_t out_stride, BatchView t, const float* __restrict__ own,
-    const int* __restrict__ plan, const float* __restrict__ shared, BatchPlan bp, int least) {
+    const int* __restrict__ plan, const float* __restrict__ shared, BatchPlan bp) {
     constexpr int kLanes  = D / 4;
-    constexpr int kGroups = kRow * kWave / kLanes;
-    __shared__ float          wsum[kMergeWaves];
-    __shared__ __attribute__((aligned(16))) float acc_s[kMergeWaves][D];
-    const int tid  = static_cast<int>(threadIdx.x);
-    const int lane = tid & (kWave - 1), wave = tid / kWave;
-    const int hq   = t.hkv * t.group;
-    const int row  = static_cast<int>(blockIdx.x) * (kMergeWaves / kRow) + wave / kRow;
-    const bool has = row < t.num_seqs * hq;
-    const int b = has ? row / hq : 0, head = has ? row % hq : 0;
+    constexpr int kGroups = kMergeWaves * kWave / kLanes;
+    constexpr int kAtOnce = 4;
+    __shared__ float                              top_s[kGroups], sum_s[kGroups];
+    __shared__ __attribute__((aligned(16))) float acc_s[kGroups][D];
+    const int tid = static_cast<int>(threadIdx.x);
+    const int hq  = t.hkv * t.group;
+    const int b = uniform(static_cast<int>(blockIdx.x) / hq), head = static_cast<int>(blockIdx.x) - b * hq;
     const int first = plan[2 * b], n_own = plan[2 * b + 1];
     const int prefix = prefix_keys(t);
     const int n_tile = bp.tile_waves != 0 ? AttnTile<D>::kN : WaveTile<D>::kN;
     const int n_pre =
-        prefix > 0 ? prefix_runs((prefix + n_tile - 1) / n_tile, bp.splits, least).live : 0;
+        prefix > 0 ? prefix_runs((prefix + n_tile - 1) / n_tile, bp.splits, bp.least).live : 0;
     const int64_t own_rows = static_cast<int64_t>(bp.slots) * hq;
     const int64_t pre_rows = static_cast<int64_t>(bp.splits) * t.num_seqs * hq;
     const int n = t.lens[b] > 0 ? n_pre + n_own : 0;
-    // Partial s of the row: its m (l and O behind it).
-    auto part = [&](int s, int64_t& rows, int64_t& at) {
-        const bool pre = s < n_pre;
-        rows = pre ? pre_rows : own_rows;
-        at   = pre ? (static_cast<int64_t>(s) * t.num_seqs + b) * hq + head
-                   : static_cast<int64_t>(first + s - n_pre) * hq + head;
-        return pre ? shared : own;
-    };
-    float top = -INFINITY;
-    for (int s = lane; s < n; s += kWave) {
-        int64_t rows, at;
-        const float* x = part(s, rows, at);
-        top            = fmaxf(top, x[at]);
-    }
-#pragma unroll
-    for (int m = 1; m < kWave; m <<= 1) {
-        top = wave_xor_max(top, m);
-    }
-    const int group = (tid % (kRow * kWave)) / kLanes, d = 4 * (tid % kLanes);
+    const int group = tid / kLanes, d = 4 * (tid % kLanes);
+
+    float top = -INFINITY, l = 0.0f;
     f32x4 acc = {};
-    float l   = 0.0f;
-#pragma unroll 4
-    for (int s = group; s < n; s += kGroups) {
-        int64_t      rows, at;
-        const float* x = part(s, rows, at);
-        const float  m = x[at];
-        const f32x4  v = *reinterpret_cast<const f32x4_a4*>(x + 2 * rows + at * D + d);
-        const float  f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-        l += f * x[rows + at];
-        acc += f * v;
-    }
-    // The groups of a wave, then the waves of a row.
+    for (int s0 = group; s0 < n; s0 += kAtOnce * kGroups) {
+        float m[kAtOnce], lv[kAtOnce];
+        f32x4 v[kAtOnce];
 #pragma unroll
-    for (int m = kLanes; m < kWave; m <<= 1) {
-        l = wave_xor_sum(l, m);
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int  s   = s0 + i * kGroups;
+            const bool pre = s < n_pre;
+            m[i]           = -INFINITY;
+            lv[i]          = 0.0f;
+            v[i]           = f32x4{};
+            if (s < n) {
+                const float*  x    = pre ? shared : own;
+                const int64_t rows = pre ? pre_rows : own_rows;
+                const int64_t at   = pre ? (static_cast<int64_t>(s) * t.num_seqs + b) * hq + head
+                                         : static_cast<int64_t>(first + s - n_pre) * hq + head;
+                m[i]  = x[at];
+                lv[i] = x[rows + at];
+                v[i]  = *reinterpret_cast<const f32x4_a4*>(x + 2 * rows + at * D + d);
+            }
+        }
+        float up = top;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            acc[i] = wave_xor_sum(acc[i], m);
+        for (int i = 0; i < kAtOnce; ++i) {
+            up = fmaxf(up, m[i]);
         }
-    }
-    if constexpr (kRow > 1) {
-        if (lane < kLanes) {
-            *reinterpret_cast<f32x4*>(&acc_s[wave][d]) = acc;
-        }
-        if (lane == 0) {
-            wsum[wave] = l;
-        }
-        __syncthreads();
-        if (wave != 0) {
-            return;
-        }
+        const float f0 = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - up);
+        l *= f0;
+        acc *= f0;
 #pragma unroll
-        for (int w = 1; w < kRow; ++w) {
-            acc += *reinterpret_cast<const f32x4*>(&acc_s[w][d]);
-            l += wsum[w];
+        for (int i = 0; i < kAtOnce; ++i) {
+            const float f = m[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[i] - up);
+            l += f * lv[i];
+            acc += f * v[i];
         }
+        top = up;
     }
-    if (has && lane < kLanes) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        u32x2       x;
-        x.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
-        x.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
-        *reinterpret_cast<u32x2*>(out + b * out_stride + static_cast<int64_t>(head) * D + d) = x;
+    *reinterpret_cast<f32x4*>(&acc_s[group][d]) = acc;
+    if (d == 0) {
+        top_s[group] = top;
+        sum_s[group] = l;
     }
+    __syncthreads();
+    if (tid >= kLanes) {
+        return;
+    }
+    float all = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+        all = fmaxf(all, top_s[g]);
+    }
+    f32x4 o     = {};
+    float total = 0.0f;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+        // (A sum of NaN alone has no maximum: it passes on by the product.)
+        const float f = top_s[g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top_s[g] - all);
+        total += f * sum_s[g];
+        o += f * *reinterpret_cast<const f32x4*>(&acc_s[g][d]);
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    u32x2       x;
+    x.x = pack_bf16x2(o[0] * inv, o[1] * inv);
+    x.y = pack_bf16x2(o[2] * inv, o[3] * inv);
+    *reinterpret_cast<u32x2*>(out + b * out_stride + static_cast<int64_t>(head) * D + d) = x;
 }
 
 // `shared`: there is a prefix (its length is known on the device only).
@@ -909,18 +969,19 @@ BatchPlan batch_plan(int num_seqs, int hq, int hkv, int head_dim, int cus, bool 
     const int group = hq / hkv, rows = num_seqs * group;
     BatchPlan p;
     p.q_blocks   = (group + 15) / 16;
-    p.tile_waves = !shared || rows <= 32 ? 0 : head_dim < 256 && rows > 128 ? 8 : 4;
+    p.tile_waves = !shared || rows <= 64 ? 0 : head_dim < 256 && rows > 128 ? 8 : 4;
     const int per_block = p.tile_waves == 0 ? 16 : 32 * p.tile_waves;
     p.row_blocks = (rows + per_block - 1) / per_block;
+    p.waves = p.tile_waves == 0 || head_dim == 256 ? 4 : 8;
+    p.least = p.tile_waves == 4 && p.waves == 8 ? 8 : 4;   // a few tiles for each wave or group of them
     // Rounds of the chip's workgroups: one for a launch of units (three or, at
     // head_dim 256, two per compute unit), half of it the prefix's; prefix tiles
-    // take one round of their own.
-    const int waves  = p.tile_waves == 0 ? 4 : p.tile_waves;
-    const int round  = cus * (p.tile_waves == 0 ? (head_dim == 256 ? 2 : 3) : head_dim == 256 ? 1 : 8 / waves);
+    // take up to one round of their own, one workgroup per compute unit.
+    const int round  = cus * (p.tile_waves != 0 ? 1 : head_dim == 256 ? 2 : 3);
     const int wgs    = p.row_blocks * hkv, most = p.tile_waves == 0 ? round / 2 : round;
     p.splits         = shared ? std::max(1, std::min(256, most / wgs)) : 0;
     const int left   = shared && p.tile_waves == 0 ? std::max(round - wgs * p.splits, round / 4) : round;
-    const int groups = (hkv * p.q_blocks + waves - 1) / waves;   // workgroups of a slot
+    const int groups = (hkv * p.q_blocks + p.waves - 1) / p.waves;   // workgroups of a slot
     p.slots = std::max(left / groups, num_seqs + std::max(8, num_seqs / 4));
     return p;
 }
@@ -936,26 +997,24 @@ hipError_t launch_batch(uint16_t* out, int64_t out_stride, const uint16_t* q, in
     int*        plan       = reinterpret_cast<int*>(partial);
     float*      own        = partial + plan_floats(t.num_seqs);
     float*      shared     = own + static_cast<std::size_t>(p.slots) * hq * (D + 2);
-    const int   waves      = p.tile_waves == 0 ? 4 : p.tile_waves;
     const int   pre        = p.row_blocks * t.hkv * p.splits;
-    const dim3  grid(static_cast<unsigned>(pre + p.slots * ((t.hkv * p.q_blocks + waves - 1) / waves)));
-    const dim3  block(static_cast<unsigned>(waves * kWave));
+    const dim3  grid(static_cast<unsigned>(pre + p.slots * ((t.hkv * p.q_blocks + p.waves - 1) / p.waves)));
+    const dim3  block(static_cast<unsigned>(p.waves * kWave));
+#define RTH_BATCH(W, G)                                                                        \
+    batch_kernel<D, W, G><<<grid, block, 0, stream>>>(q, q_stride, t, own, plan, shared, p, pre, \
+                                                      scale_log2)
     if (p.tile_waves == 0) {
-        batch_kernel<D, 4, false><<<grid, block, 0, stream>>>(q, q_stride, t, own, plan, shared, p, pre, scale_log2);
+        RTH_BATCH(4, 0);
+    } else if constexpr (D == 256) {
+        RTH_BATCH(4, 1);
     } else if (p.tile_waves == 4) {
-        batch_kernel<D, 4, true><<<grid, block, 0, stream>>>(q, q_stride, t, own, plan, shared, p, pre, scale_log2);
-    } else if constexpr (D < 256) {
-        batch_kernel<D, 8, true><<<grid, block, 0, stream>>>(q, q_stride, t, own, plan, shared, p, pre, scale_log2);
-    }
-    const int rows  = t.num_seqs * hq;
-    const int least = p.tile_waves == 0 ? kUnitTiles : kPrefixTiles;
-    if (rows >= 1024) {
-        batch_merge_kernel<D, 1><<<dim3(static_cast<unsigned>((rows + kMergeWaves - 1) / kMergeWaves)),
-                                   kMergeWaves * kWave, 0, stream>>>(out, out_stride, t, own, plan, shared, p, least);
+        RTH_BATCH(4, 2);
     } else {
-        batch_merge_kernel<D, kMergeWaves><<<dim3(static_cast<unsigned>(rows)), kMergeWaves * kWave, 0, stream>>>(
-            out, out_stride, t, own, plan, shared, p, least);
+        RTH_BATCH(8, 1);
     }
+#undef RTH_BATCH
+    batch_merge_kernel<D><<<dim3(static_cast<unsigned>(t.num_seqs * hq)), kMergeWaves * kWave, 0, stream>>>(
+        out, out_stride, t, own, plan, shared, p);
     return hipGetLastError();
 }
 
