@@ -162,12 +162,52 @@ __global__ __launch_bounds__(kW * kWave, D < 256 ? 2 : 1) void flash_packed_kern
         }
     };
 
+    // Row `x` of the wave's 32 (those that exist) in q or out: whole rows of D
+    // elements, kRowLanes lanes each, kRowsAt rows at once.
+    constexpr int kRowLanes = D / 8, kRowsAt = kWave / kRowLanes, kRowSteps = 32 / kRowsAt;
+    constexpr int kRowPitch = 2 * D + 16;
+    const int     have  = min(rows - wr0, 32);   // (negative: an idle wave)
+    const int     token = uniform(wr0 / group), left = wr0 - token * group;
+    const float   part  = 1.0f / static_cast<float>(group);
+    auto row_at = [&](int x, int64_t stride) {
+        // Exact: (left + x + 1/2) / group lies at least 1 / (2 group) from a whole number.
+        const int n = static_cast<int>((static_cast<float>(left + x) + 0.5f) * part);
+        return (row0 + token + n) * stride + (static_cast<int64_t>(kvh) * group + (left + x - n * group)) * D;
+    };
+
     load(kh, k_stride, 0, kreg);
     QueryRows<D, false, kW == 8> rq;
     rq.lane = lane;
-    rq.load_q(q + (row0 + my_tok) * q_stride +
-              (static_cast<int64_t>(kvh) * group + (my_row - my_tok * group)) * D);
-    load(vh, v_stride, 0, vreg);
+    if constexpr (kW == 4) {
+        // q in whole rows, to the operand layout through LDS (a lane's own row in
+        // pieces of 32 bytes: 64 x 128 tokens x 32 heads 63 us, now QQ).
+        uint8_t* area = lds + T::v_at(0) + wave * 32 * kRowPitch;
+        static_assert(kW * 32 * kRowPitch <= 2 * T::kV, "the waves' rows fit the V tiles");
+        const int r = lane / kRowLanes, chunk = lane % kRowLanes;
+        u32x4     x[kRowSteps];
+        if (have > 0) {
+#pragma unroll
+            for (int s = 0; s < kRowSteps; ++s) {
+                x[s] = *reinterpret_cast<const u32x4*>(
+                    q + row_at(min(s * kRowsAt + r, have - 1), q_stride) + 8 * chunk);
+            }
+#pragma unroll
+            for (int s = 0; s < kRowSteps; ++s) {
+                *reinterpret_cast<u32x4*>(area + (s * kRowsAt + r) * kRowPitch + 16 * chunk) = x[s];
+            }
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+                rq.qf[c] = *reinterpret_cast<const bf16x8*>(area + col * kRowPitch + 32 * c + 16 * h);
+            }
+        }
+        load(vh, v_stride, 0, vreg);
+        __syncthreads();
+    } else {
+        if (have > 0) {
+            rq.load_q(q + row_at(min(col, have - 1), q_stride));
+        }
+        load(vh, v_stride, 0, vreg);
+    }
     rq.clear();
     store(T::k_at(0), T::kKPitch, kreg);
     // The first step multiplies zero weights with the "tile before".
@@ -208,27 +248,36 @@ __global__ __launch_bounds__(kW * kWave, D < 256 ? 2 : 1) void flash_packed_kern
         }
         half(std::integral_constant<int, 1>{}, T::k_at(i + 1), T::v_at(i));
     }
-    if (mine < 0) {
-        return;
-    }
     if (mine == 2 * n_tiles) {
         rq.last(lds + T::v_at(n_tiles - 1) + 32 * T::kVPitch);
     }
+    // O to bf16 rows in LDS, stored as whole rows.
     const float inv = 1.0f / wave_xor_sum(rq.l_run, 32);
-    const int   r   = again(wr0 + col);
-    if (r < rows) {
-        const int64_t t    = r / group;
-        uint16_t*     orow = out + (row0 + t) * out_stride +
-                         (static_cast<int64_t>(kvh) * group + (r - t * group)) * D;
+    __syncthreads();   // the tiles are done with
+    if (mine < 0) {
+        return;
+    }
+    static_assert(kW * 32 * kRowPitch <= T::kBytes, "the waves' rows fit the tiles");
+    const int ln   = again(lane);
+    uint8_t*  area = lds + wave * 32 * kRowPitch;
+    uint8_t*  to   = area + (ln & 31) * kRowPitch + 8 * (ln >> 5);
 #pragma unroll
-        for (int b = 0; b < D / 32; ++b) {
+    for (int b = 0; b < D / 32; ++b) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                u32x2 x;
-                x.x = pack_bf16x2(rq.o[b][4 * g] * inv, rq.o[b][4 * g + 1] * inv);
-                x.y = pack_bf16x2(rq.o[b][4 * g + 2] * inv, rq.o[b][4 * g + 3] * inv);
-                *reinterpret_cast<u32x2*>(orow + 32 * b + 8 * g + 4 * h) = x;
-            }
+        for (int g = 0; g < 4; ++g) {
+            u32x2 x;
+            x.x = pack_bf16x2(rq.o[b][4 * g] * inv, rq.o[b][4 * g + 1] * inv);
+            x.y = pack_bf16x2(rq.o[b][4 * g + 2] * inv, rq.o[b][4 * g + 3] * inv);
+            *reinterpret_cast<u32x2*>(to + 64 * b + 16 * g) = x;
+        }
+    }
+    const int r = ln / kRowLanes, chunk = ln % kRowLanes;
+#pragma unroll
+    for (int s = 0; s < kRowSteps; ++s) {
+        const int x = s * kRowsAt + r;
+        if (x < have) {
+            *reinterpret_cast<u32x4*>(out + row_at(x, out_stride) + 8 * chunk) =
+                *reinterpret_cast<const u32x4*>(area + x * kRowPitch + 16 * chunk);
         }
     }
 }
