@@ -343,8 +343,8 @@ int rth_rmsnorm_lanes(int hidden_dim);
  * b holds rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (cu_seqlens: num_seqs + 1
  * device ints, ascending; bounds past num_rows are taken as num_rows). Rows
  * behind the last sequence are neither read nor written. Row strides are in
- * elements, multiples of 8, at least heads * head_dim (so q, k and v may be
- * slices of one projection's rows). Rows of q, k, v and out start 16-byte aligned.
+ * elements, multiples of 8, at least heads * head_dim and at most 2^24 (so q, k
+ * and v may be slices of one projection's rows). Rows of q, k, v and out start 16-byte aligned.
  *
  * Block tables of a batch: [num_seqs, table_blocks] device ints; entry i of row
  * b is the page of positions i * block_size .. (i + 1) * block_size - 1 of

@@ -209,8 +209,9 @@ int check_batch(int num_seqs) {
 }
 
 int check_row_stride(int64_t stride, int64_t heads, int head_dim, const char* name) {
-    RTH_REQUIRE(stride >= heads * head_dim && stride % 8 == 0,
-                std::string(name) + " must be a multiple of 8 and at least heads * head_dim");
+    RTH_REQUIRE(stride >= heads * head_dim && stride % 8 == 0 && stride <= (1 << 24),
+                std::string(name) + " must be a multiple of 8, at least heads * head_dim and at "
+                                    "most 2^24");
     return RTH_OK;
 }
 

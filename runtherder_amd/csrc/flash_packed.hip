@@ -147,12 +147,25 @@ __global__ __launch_bounds__(kW * kWave, D < 256 ? 2 : 1) void flash_packed_kern
     const uint16_t* vh   = v + row0 * v_stride + static_cast<int64_t>(kvh) * D;
     const int       crow = tid / kCpr, cchunk = tid % kCpr;
     u32x4 kreg[kSteps], vreg[kSteps];
-    // A row past the sequence's last repeats it: every key past a row's own is masked.
+    // Tile i of x: a scalar base and a 32-bit offset per lane. A row past the
+    // sequence's last repeats it: every key past a row's own is masked.
     auto load = [&](const uint16_t* x, int64_t stride, int i, u32x4 (&reg)[kSteps]) {
+        const uint8_t* base = reinterpret_cast<const uint8_t*>(x + static_cast<int64_t>(i) * T::kN * stride);
+        const uint32_t pitch = 2u * static_cast<uint32_t>(stride);
+        const int      last  = n - 1 - i * T::kN;
+        if (last >= T::kN - 1) {
+            const uint32_t off = static_cast<uint32_t>(crow) * pitch + 16u * static_cast<uint32_t>(cchunk);
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const int64_t r = min(i * T::kN + s * kCopy + crow, n - 1);
-            reg[s]          = *reinterpret_cast<const u32x4*>(x + r * stride + 8 * cchunk);
+            for (int s = 0; s < kSteps; ++s) {
+                reg[s] = *reinterpret_cast<const u32x4*>(base + static_cast<int64_t>(s * kCopy) * pitch + off);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                const int r = min(s * kCopy + crow, last);
+                reg[s] = *reinterpret_cast<const u32x4*>(
+                    base + (static_cast<uint32_t>(r) * pitch + 16u * static_cast<uint32_t>(cchunk)));
+            }
         }
     };
     auto store = [&](uint32_t to, int pitch, const u32x4 (&reg)[kSteps]) {
