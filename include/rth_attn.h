@@ -381,7 +381,9 @@ int rth_kv_append_fp8_batch(uint8_t* k_cache, uint8_t* v_cache, float* k_scale, 
  * others lie in the sequence's own row of block_tables, at their own positions
  * (so tables that rth_pages_fork made can be passed whole, with any one of
  * their rows as prefix_table). prefix_table and prefix_len NULL: nothing is shared. lens[b] <= 0:
- * an unused slot, its output row is zeros. Keys past a table's end, and keys whose
+ * an unused slot, its output row is zeros. A sequence shorter than the prefix sees
+ * its lens[b] keys of it (where the others are finite: the rows of a kv head are one
+ * product, in which a NaN or an infinity times a weight of 0 is a NaN). Keys past a table's end, and keys whose
  * table entry names no page, are left out. head_dim 64, 128, 256; any Hq / Hkv.
  * partial: rth_batch_scratch_floats floats, 16-byte aligned, no
  * initialization needed, not shared by calls that overlap (graphs included). */
@@ -422,8 +424,7 @@ int rth_pages_reserve(int* refs, int* work, int* status, int num_blocks, int blo
  * filled, a page of its own with a copy of the filled rows of every layer.
  * dst_tables [num_children, table_blocks] and dst_lens are written whole and
  * may not overlap the source's; what they held before is to be freed first. A
- * parent outside 0 .. num_src - 1 gives an empty child. num_children <=
- * min(4096, num_blocks). */
+ * parent outside 0 .. num_src - 1 gives an empty child. num_children <= 4096. */
 int rth_pages_fork(uint8_t* k, uint8_t* v, float* k_scale, float* v_scale, int num_layers,
                    int num_blocks, int block_size, int num_kv_heads, int head_dim, int* refs,
                    int* work, int* status, int* dst_tables, int* dst_lens,

@@ -34,7 +34,7 @@ __device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
 // V^T is read (ds_read_b64_tr_b16) in the scores' key order. Softmax in base 2,
 // fp32, with a lazy reference maximum: it moves at the first keys, and when a
 // row's sum of 32 weights passes 2^20; one reference for the sum and for O, so
-// the result does not depend on it. P is rounded to bf16 (half a step, 2^-9 of
+// the result does not depend on it. P is rounded to bf16 (half a step, 2^-8 of
 // each weight) for the matrix product, the row sum takes the fp32 values.
 //
 // Software pipelined by halves of a tile (32 keys): one step does the softmax
@@ -218,14 +218,18 @@ struct QueryRows {
                 }
             }
         }
-        if (__any(start || !(sum[0] + sum[1] <= 0x1p20f))) {
+        const bool high = !(sum[0] + sum[1] <= 0x1p20f);
+        if (__any(start || high)) {
             float top = x[0];
 #pragma unroll
             for (int e = 1; e < 16; ++e) {
                 top = fmaxf(top, x[e]);
             }
-            top               = wave_xor_max(top, 32);
-            const float up    = start ? (top == -INFINITY ? 0.0f : top) : fmaxf(top, 0.0f);
+            top = wave_xor_max(top, 32);
+            // (Rows that need no new reference keep theirs: a row's result does not
+            // depend on the others of its wave.)
+            const bool  need  = wave_xor_max(high ? 1.0f : 0.0f, 32) != 0.0f;
+            const float up    = start ? (top == -INFINITY ? 0.0f : top) : need ? fmaxf(top, 0.0f) : 0.0f;
             const float alpha = start ? 1.0f : __builtin_amdgcn_exp2f(-up);
             m_ref += up;
             l_run *= alpha;

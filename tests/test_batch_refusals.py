@@ -89,7 +89,7 @@ def test_page_slabs(change, says):
     ("rth_pages_reserve", RESERVE, dict(seqs=4097), "num_seqs"), ("rth_pages_reserve", RESERVE, dict(width=0), "table_blocks"),
     ("rth_pages_fork", FORK, dict(parents=None), "parents"), ("rth_pages_fork", FORK, dict(status=None), "status"),
     ("rth_pages_fork", FORK, dict(dt=2 * P), "of its own"), ("rth_pages_fork", FORK, dict(dl=2 * P), "of its own"),
-    ("rth_pages_fork", FORK, dict(kids=0), "num_children"), ("rth_pages_fork", FORK, dict(kids=17), "num_children"),
+    ("rth_pages_fork", FORK, dict(kids=0), "num_children"), ("rth_pages_fork", FORK, dict(kids=4097), "num_children"),
     ("rth_pages_fork", FORK, dict(src=0), "num_seqs"),
     ("rth_pages_free", FREE, dict(lens=None), "lens"), ("rth_pages_free", FREE, dict(tables=None), "block_tables"),
     ("rth_pages_free", FREE, dict(blocks=0), "num_blocks"),

@@ -23,7 +23,7 @@ class Batch:
         shared = -(-prefix // block)
         blocks = shared + sum(holds) + 2
         g = torch.Generator().manual_seed(seed)
-        pages = torch.randperm(blocks, generator=g).int()
+        pages = 1 + torch.randperm(blocks - 1, generator=g).int()   # the first page holds NaN
         width = max(1, whole + max(holds))
         t = torch.full((len(own), width), -1, dtype=torch.int32)
         t[:, :whole] = pages[:whole]
@@ -164,6 +164,28 @@ def test_missing_pages_are_left_out():
         sc[0, rest.to(DEV)] = s[0].item()
         (t.kv[0] if x == 0.5 else t.kv[1])[rest] = dequantize(codes, s)[0]
     step("batch decode missing pages")
+    out = t.run()
+    sync()
+    t.check(out.cpu())
+
+
+@pytest.mark.parametrize("seqs", [2, 20, 70])
+def test_missing_prefix_pages_with_many_rows(seqs):
+    """A prefix page that is not there, where the first page holds NaN, in each of the
+    ways a prefix is multiplied (few rows, blocks of 128, of 256)."""
+    t = Batch([3] * seqs, 700, 16, 2, 128, 32, 3450)
+    pt = t.prefix_table.cpu()
+    for c, s in ((t.cache.k, t.cache.k_scale), (t.cache.v, t.cache.v_scale)):
+        if not (pt == 0).any() and not (t.tables == 0).any():
+            c[0, :32], s[0, :32] = 0x7f, math.nan
+    pt[[0, 5, 6, 21]] = -1
+    t.prefix_table = pt.to(DEV)
+    for b in range(seqs):
+        p = torch.arange(t.lens[b])
+        block = p // 32
+        gone = (p < 700) & ((block == 0) | (block == 5) | (block == 6) | (block == 21))
+        t.at[b] = t.at[b][~gone]
+    step(f"batch decode missing prefix pages seqs={seqs}")
     out = t.run()
     sync()
     t.check(out.cpu())

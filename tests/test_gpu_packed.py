@@ -96,6 +96,22 @@ def test_score_ranges():
         assert_attention(out[t], want, weight, score_size(q[t], k[:t + 1], d ** -0.5))
 
 
+def test_a_prompt_is_the_same_in_every_batch():
+    """Bit for bit, whatever the batch, its padding and its workgroups' width."""
+    for hq, hkv, d in ((32, 8, 128), (6, 2, 64), (4, 4, 256)):
+        n = 333
+        q, k, v = (normal((4300, h, d), 610 + h, 4.0) for h in (hq, hkv, hkv))
+        alone = run(q[:n].to(DEV), k[:n].to(DEV), v[:n].to(DEV), ints([0, n])).cpu()
+        front = run(q.to(DEV), k.to(DEV), v.to(DEV), ints([0, 4300])).cpu()
+        back = torch.cat([q[-100:], q[:n], q[:7]]), torch.cat([k[-100:], k[:n], k[:7]]), \
+            torch.cat([v[-100:], v[:n], v[:7]])
+        step(f"packed batch against alone hq={hq} d={d}")
+        there = run(*(t.to(DEV) for t in back), ints([0, 100, 100 + n])).cpu()
+        sync()
+        assert torch.equal(front[:n], alone)
+        assert torch.equal(there[100:100 + n], alone)
+
+
 def test_repeats_bit_for_bit_and_on_a_stream():
     q, k, v = (normal((700, h, 128), 600 + h).to(DEV) for h in (16, 4, 4))
     cu = ints([0, 300, 301, 700])
@@ -106,3 +122,35 @@ def test_repeats_bit_for_bit_and_on_a_stream():
     run(q, k, v, cu, out=b, stream=s)
     s.synchronize()
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("hq,hkv,d,n", [(8, 2, 128, 200), (4, 4, 64, 150), (4, 2, 256, 90), (32, 8, 128, 4200)])
+def test_what_a_row_does_not_see_leaves_no_trace(hq, hkv, d, n):
+    """NaN and infinities in K and V: rows in front of them are those of a clean batch, bit
+    for bit; the rows that see them have what the formula gives."""
+    at = n - 61
+    q, k, v = (normal((n + 40, h, d), 700 + h) for h in (hq, hkv, hkv))
+    clean = run(q.to(DEV), k.to(DEV), v.to(DEV), ints([0, n, n + 40])).cpu()
+    v[at, 0, 5] = math.inf
+    v[at + 3, 0, 6] = -math.inf
+    v[at + 7, 0, 7] = math.nan
+    v[at + 9, 0, 5] = -math.inf            # with the one before: NaN
+    v[n - 1, 0, 8] = math.nan              # the last row, which fills up the tile
+    k[at + 20, hkv - 1, :] = math.nan
+    k[n - 1, 0, 3] = math.inf
+    step(f"packed non-finite hq={hq} hkv={hkv} d={d}")
+    got = run(q.to(DEV), k.to(DEV), v.to(DEV), ints([0, n, n + 40])).cpu()
+    sync()
+    assert torch.equal(got[:at], clean[:at]) and torch.equal(got[n:], clean[n:])
+    assert torch.isfinite(got[n:].float()).all()
+    g = hq // hkv
+    f = got.float()
+    own = f[:, :g]                          # the heads of kv head 0
+    assert (own[at:n - 1, :, 6][:3] == clean.float()[at:at + 3, :g, 6]).all()
+    assert (own[at:at + 9, :, 5] == math.inf).all() and torch.isnan(own[at + 9:n - 1, :, 5]).all()
+    assert (own[at + 3:n - 1, :, 6] == -math.inf).all()
+    assert torch.isfinite(own[at:at + 7, :, 7]).all() and torch.isnan(own[at + 7:n - 1, :, 7]).all()
+    if hkv > 1:
+        other = f[:, (hkv - 1) * g:]
+        assert torch.equal(got[:at + 20, (hkv - 1) * g:], clean[:at + 20, (hkv - 1) * g:])
+        assert torch.isnan(other[at + 20:n]).all()
