@@ -39,4 +39,19 @@ struct KVSlabs {
     }
 };
 
+// One layer of a paged cache with the block tables of a batch ([num_seqs,
+// table_blocks], entries < 0 hold no page), as PagedKVCache::batch_view makes it.
+// No reference counterpart.
+struct KVBatchView {
+    const __hip_fp8_e4m3* k;
+    const __hip_fp8_e4m3* v;
+    const float*          k_scale;
+    const float*          v_scale;
+    const int*            block_tables;
+    int                   table_blocks;
+    int                   num_seqs;
+    int                   num_blocks;
+    int                   block_size;
+};
+
 }  // namespace runtherder::attention

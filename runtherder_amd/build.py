@@ -100,18 +100,19 @@ def build_oracle(verbose: bool = False) -> Path:
     return ROOT / "oracle" / "librth_oracle.so"
 
 
-def build_cpp_tests(verbose: bool = False) -> Path:
-    """Compile the C++ drop-in test driver against the C++ layer."""
+def build_cpp_tests(verbose: bool = False) -> list[Path]:
+    """Compile the C++ test drivers (drop-in and batch) against the C++ layer."""
     out_dir = ROOT / "tests" / "cpp" / "bin"
     out_dir.mkdir(parents=True, exist_ok=True)
-    exe = out_dir / "test_backend"
-    _run([HIPCC, *DEVICE_FLAGS, "-x", "hip", str(ROOT / "tests" / "cpp" / "test_backend.cpp"),
-          f"-I{ROOT / 'oracle'}", "-o", str(exe), f"-L{LIB_DIR}", "-lruntherder_attn_cpp",
-          "-lruntherder_attn", f"-L{ROOT / 'oracle'}", "-lrth_oracle",
-          f"-Wl,-rpath,{LIB_DIR}", f"-Wl,-rpath,{ROOT / 'oracle'}",
-          "-Wl,-rpath,$ORIGIN/../../../runtherder_amd/lib",
-          "-Wl,-rpath,$ORIGIN/../../../oracle"], verbose)
-    return exe
+    exes = [out_dir / "test_backend", out_dir / "test_batch"]
+    for exe in exes:
+        _run([HIPCC, *DEVICE_FLAGS, "-x", "hip", str(ROOT / "tests" / "cpp" / f"{exe.name}.cpp"),
+              f"-I{ROOT / 'oracle'}", "-o", str(exe), f"-L{LIB_DIR}", "-lruntherder_attn_cpp",
+              "-lruntherder_attn", f"-L{ROOT / 'oracle'}", "-lrth_oracle",
+              f"-Wl,-rpath,{LIB_DIR}", f"-Wl,-rpath,{ROOT / 'oracle'}",
+              "-Wl,-rpath,$ORIGIN/../../../runtherder_amd/lib",
+              "-Wl,-rpath,$ORIGIN/../../../oracle"], verbose)
+    return exes
 
 
 if __name__ == "__main__":

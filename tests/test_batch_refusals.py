@@ -1,5 +1,7 @@
 """What the batch operators refuse, before anything reaches the GPU (CPU only)."""
 import ctypes
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
@@ -132,3 +134,21 @@ def test_python_checks():
             cache.append_batch(layer, host, host, i, i)
         with pytest.raises(ValueError):
             cache.batch_view(layer, i)
+
+
+@pytest.mark.parametrize("header,check", [
+    ("runtherder/kernels/batch.h", "static_assert(sizeof(&runtherder::kernels::flash_decode_batch_bf16) > 0);"),
+    ("runtherder/attention/batch.h",
+     "static_assert(std::is_constructible_v<runtherder::attention::BatchAttention, "
+     "const runtherder::attention::AttnConfig&, int>);"),
+    ("runtherder/engine/page_pool.h",
+     "static_assert(std::is_same_v<decltype(std::declval<const runtherder::engine::PagedKVCache&>()"
+     ".batch_view(0, nullptr, 1, 1)), runtherder::attention::KVBatchView>);"),
+])
+def test_cpp_headers_stand_alone(header, check):
+    root = Path(__file__).resolve().parents[1]
+    src = f"#include <{header}>\n#include <type_traits>\n#include <utility>\n{check}\nint main() {{ return 0; }}\n"
+    res = subprocess.run(["/opt/rocm/bin/hipcc", "-std=c++20", "-fsyntax-only", "-Wall", "-x", "hip",
+                          f"-I{root / 'include'}", "--offload-arch=gfx950", "-"],
+                         input=src, capture_output=True, text=True)
+    assert res.returncode == 0 and "warning" not in res.stderr, res.stderr[-3000:]
