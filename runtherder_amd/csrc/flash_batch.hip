@@ -104,12 +104,27 @@ __device__ __forceinline__ int wave_exclusive_i(int v, int lane, int& total) {
     return x - v;
 }
 
+// How a launch is split. Prefix: splits of the keys for each block of rows;
+// own keys: slots of runs.
+struct BatchPlan {
+    int q_blocks;      // blocks of 16 q heads of a kv head
+    int slots;
+    int waves;         // of a workgroup
+    int splits;        // of the prefix
+    int row_blocks;    // of the prefix's rows, of a kv head
+    int least, most;   // tiles of a split: least, and up to most of them before the second
+                       // half of the splits is used (a partial costs as much as some tiles)
+    int tile_waves;    // 0: prefix_units takes the prefix; else the waves of a block of prefix_tiles's rows
+};
+
 // Units of one prefix split, and how many splits have keys.
 struct PrefixRuns {
     int per, live;
 };
-__device__ __forceinline__ PrefixRuns prefix_runs(int tiles, int num_splits, int least) {
-    const int per = max((tiles + num_splits - 1) / num_splits, least);
+__device__ __forceinline__ PrefixRuns prefix_runs(int tiles, const BatchPlan& p) {
+    const int half = max(p.splits / 2, 1);
+    const int want = min(max((tiles + half - 1) / half, p.least), p.most);
+    const int per  = max((tiles + p.splits - 1) / p.splits, want);
     return {per, (tiles + per - 1) / per};
 }
 
@@ -453,18 +468,6 @@ struct WaveRows {
     }
 };
 
-// How a launch is split. Prefix: splits of the keys for each block of rows;
-// own keys: slots of runs.
-struct BatchPlan {
-    int q_blocks;      // blocks of 16 q heads of a kv head
-    int slots;
-    int waves;         // of a workgroup
-    int splits;        // of the prefix
-    int row_blocks;    // of the prefix's rows, of a kv head
-    int least;         // tiles of a split, if there are as many
-    int tile_waves;    // 0: prefix_units takes the prefix; else the waves of a block of prefix_tiles's rows
-};
-
 // Workgroup `bid` of the prefix, few rows: (split, block of 16 rows, kv head), the
 // waves taking the split's tiles in turn.
 template <int D, int kW>
@@ -477,7 +480,7 @@ __device__ __forceinline__ void prefix_units(uint8_t* lds, int bid, int prefix,
     const int wave = uniform(tid / kWave), lane = tid & (kWave - 1), col = lane & 15;
     const int hq   = t.hkv * t.group;
     const int tiles = (prefix + T::kN - 1) / T::kN;
-    const PrefixRuns runs = prefix_runs(tiles, bp.splits, bp.least);
+    const PrefixRuns runs = prefix_runs(tiles, bp);
     const int at = uniform(bid / t.hkv), kvh = bid - at * t.hkv;
     const int split = uniform(at / bp.row_blocks), rb = at - split * bp.row_blocks;
     if (split >= runs.live) {
@@ -591,7 +594,7 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D> (&sm)[kG], int bid, in
     constexpr bool kSome = kCopy > T::kN;  // more threads than chunks
     const int num_splits = bp.splits;
     const int tiles  = (prefix + T::kN - 1) / T::kN;
-    const PrefixRuns runs  = prefix_runs(tiles, num_splits, bp.least);
+    const PrefixRuns runs  = prefix_runs(tiles, bp);
     const int at0   = uniform(bid / t.hkv), hb = bid - at0 * t.hkv;
     const int split = uniform(at0 / bp.row_blocks), blk = at0 - split * bp.row_blocks;
     if (split >= runs.live) {
@@ -894,12 +897,17 @@ __global__ __launch_bounds__(kMergeWaves * kWave) void batch_merge_kernel(
     __shared__ __attribute__((aligned(16))) float acc_s[kGroups][D];
     const int tid = static_cast<int>(threadIdx.x);
     const int hq  = t.hkv * t.group;
-    const int b = uniform(static_cast<int>(blockIdx.x) / hq), head = static_cast<int>(blockIdx.x) - b * hq;
+    // Rows whose prefix partials the same XCD wrote (prefix_tiles's kv heads): they may be
+    // in its L2 still (32 sequences after 8192 keys 26.9 -> 24.7 us, 64 after 2048 27.1 -> 24.3).
+    const int wg = static_cast<int>(blockIdx.x);
+    const int xcds = bp.tile_waves != 0 && (t.hkv & 7) == 0 ? 8 : 1;
+    const int at0 = wg / xcds, part = hq / xcds;
+    const int b = uniform(at0 / part), head = at0 - b * part + (wg - at0 * xcds) * part;
     const int first = plan[2 * b], n_own = plan[2 * b + 1];
     const int prefix = prefix_keys(t);
     const int n_tile = bp.tile_waves != 0 ? AttnTile<D>::kN : WaveTile<D>::kN;
     const int n_pre =
-        prefix > 0 ? prefix_runs((prefix + n_tile - 1) / n_tile, bp.splits, bp.least).live : 0;
+        prefix > 0 ? prefix_runs((prefix + n_tile - 1) / n_tile, bp).live : 0;
     const int64_t own_rows = static_cast<int64_t>(bp.slots) * hq;
     const int64_t pre_rows = static_cast<int64_t>(bp.splits) * t.num_seqs * hq;
     const int n = t.lens[b] > 0 ? n_pre + n_own : 0;
@@ -982,7 +990,12 @@ BatchPlan batch_plan(int num_seqs, int hq, int hkv, int head_dim, int cus, bool 
     const int per_block = p.tile_waves == 0 ? 16 : 32 * p.tile_waves;
     p.row_blocks = (rows + per_block - 1) / per_block;
     p.waves = p.tile_waves == 0 || head_dim == 256 ? 4 : 8;
-    p.least = p.tile_waves == 4 && p.waves == 8 ? 8 : 4;   // a few tiles for each wave or group of them
+    // A tile per group of waves for short prefixes (32 sequences after 1000 keys, tiles
+    // of a split 8 -> 2: 23 -> 17 us), eight before more than half the splits write partials
+    // (64 after 8192, 4 -> 8: 39 -> 34; head_dim 256, whose tiles take twice as
+    // long, 64 after 8000, 4 -> 8: 45 -> 48).
+    p.least = p.tile_waves != 0 ? p.waves / p.tile_waves : 3;
+    p.most  = p.tile_waves != 0 && head_dim == 256 ? 4 : 8;
     // Rounds of the chip's workgroups: one for a launch of units (three or, at
     // head_dim 256, two per compute unit), half of it the prefix's; prefix tiles
     // take up to one round of their own, one workgroup per compute unit.
