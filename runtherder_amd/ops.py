@@ -322,7 +322,12 @@ def _need_rows(t: torch.Tensor, heads: int, head_dim: int, name: str, device: in
         raise ValueError(f"{name} must be [rows, {heads}, {head_dim}], got {tuple(shape)}")
     if stride[2] != 1 or (stride[1] != head_dim and heads > 1):
         raise TypeError(f"{name}: a row's heads must be contiguous")
-    return stride[0] if shape[0] > 1 else max(stride[0], heads * head_dim)
+    return stride[0] if shape[0] > 1 else heads * head_dim
+
+
+def _need_here(t: torch.Tensor, name: str, device: int) -> None:
+    if t.get_device() != device:
+        raise TypeError(f"{name} must be on the current device")
 
 
 def _need_len(t: torch.Tensor, n: int, name: str, device: int) -> None:
@@ -628,8 +633,7 @@ class PagedKVCache:
         (cu_seqlens), or one row per sequence, at at_pos[b] of sequence b."""
         if not 0 <= layer < self.num_layers:
             raise ValueError("KVCache append layer out of range")
-        if not self.k.is_cuda:
-            raise TypeError("the cache must be on the device")
+        _need_here(self.k, "the cache", _current_device())
         rows = layer * self.num_blocks * self.block_size * self.num_kv_heads
         _append_batch(self.k.data_ptr() + rows * self.head_dim,
                       self.v.data_ptr() + rows * self.head_dim,
@@ -656,6 +660,7 @@ class PagedKVCache:
         """Copies page src[i] to page dst[i] in every layer. The dst pages are
         distinct and none of them is a src page."""
         dev = _current_device()
+        _need_here(self.k, "the cache", dev)
         _need_on(src, torch.int32, "src", dev)
         n = src.numel()
         _need_len(dst, n, "dst", dev)
@@ -691,14 +696,20 @@ class PagePool:
         """Block tables without pages."""
         return torch.full((num_seqs, table_blocks), -1, dtype=torch.int32, device=self.device)
 
+    def _here(self):
+        dev = _current_device()
+        _need_here(self.refs, "the pool", dev)
+        return dev
+
     def _of(self, cache):
         if cache.num_blocks != self.num_blocks or cache.block_size != self.block_size:
             raise ValueError("the pool and the cache differ in their blocks")
+        _need_here(cache.k, "the cache", self._here())
 
     def reserve(self, block_tables, lens, n_new, stream=None):
         """Pages for positions lens[b] .. lens[b] + n_new[b] - 1 of sequence b,
         where its table row has none yet."""
-        dev, seqs = _current_device(), lens.numel()
+        dev, seqs = self._here(), lens.numel()
         _need_on(lens, torch.int32, "lens", dev)
         _need_len(n_new, seqs, "n_new", dev)
         width = _need_tables(block_tables, seqs, "block_tables", dev)
@@ -729,7 +740,7 @@ class PagePool:
     def free(self, block_tables, lens, drop=None, stream=None):
         """Frees the sequences with drop[b] != 0 (None: all): their pages lose
         one reference, their table rows hold none, their lengths are 0."""
-        dev, seqs = _current_device(), lens.numel()
+        dev, seqs = self._here(), lens.numel()
         _need_on(lens, torch.int32, "lens", dev)
         width = _need_tables(block_tables, seqs, "block_tables", dev)
         if drop is not None:
@@ -927,6 +938,8 @@ class BatchAttention:
             raise ValueError(f"{seqs} sequences: this backend was made for {self.max_seqs}")
         if kv.num_kv_heads != c.num_kv_heads or kv.head_dim != c.head_dim:
             raise ValueError("the view and the configuration differ in their kv heads")
+        dev = _current_device()
+        _need_here(kv.k, "the view", dev); _need_here(self.partial, "the scratch", dev)
         _decode_batch(out, q, kv.k, kv.v, kv.k_scale, kv.v_scale, tables, width, kv.num_blocks,
                       kv.block_size, lens, self.partial, c.num_q_heads, c.num_kv_heads, c.head_dim,
                       c.scale, prefix_table, prefix_len, stream)

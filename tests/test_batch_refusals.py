@@ -136,6 +136,18 @@ def test_python_checks():
             cache.batch_view(layer, i)
 
 
+def test_a_cache_or_pool_elsewhere():
+    """Every tensor behind a call lies on the current device: a cache's, a pool's, a view's."""
+    rows = torch.zeros((2, 1, 8), dtype=torch.bfloat16)
+    i, pages = torch.zeros(2, dtype=torch.int32), torch.zeros((2, 2), dtype=torch.int32)
+    cache, pool = R.PagedKVCache(1, 4, 32, 1, 8, device="cpu"), R.PagePool(4, 32, device="cpu")
+    for call in (lambda: cache.append_batch(0, rows, rows, i, pages), lambda: cache.copy_pages(i, i),
+                 lambda: pool.reserve(pages, i, i), lambda: pool.free(pages, i),
+                 lambda: pool.fork(cache, pages, i, pages, i, i), lambda: pool.compact(cache, pages)):
+        with pytest.raises(TypeError, match="current device"):
+            call()
+
+
 @pytest.mark.parametrize("header,check", [
     ("runtherder/kernels/batch.h", "static_assert(sizeof(&runtherder::kernels::flash_decode_batch_bf16) > 0);"),
     ("runtherder/attention/batch.h",

@@ -154,3 +154,14 @@ def test_what_a_row_does_not_see_leaves_no_trace(hq, hkv, d, n):
         other = f[:, (hkv - 1) * g:]
         assert torch.equal(got[:at + 20, (hkv - 1) * g:], clean[:at + 20, (hkv - 1) * g:])
         assert torch.isnan(other[at + 20:n]).all()
+
+
+def test_one_row_of_any_stride():
+    """The stride of a single row is no part of the call."""
+    wide = normal((3, 1001), 5).to(DEV)
+    q, k, v = wide[:1, :256].view(1, 2, 128), wide[:1, 256:384].view(1, 1, 128), wide[:1, 384:512].view(1, 1, 128)
+    out = torch.zeros((1, 2, 128), dtype=torch.bfloat16, device=DEV)
+    step("one row")
+    R.flash_packed_bf16(out, q, k, v, ints([0, 1]), 2, 1, 128, 0.1)
+    sync()
+    assert torch.equal(out, v.expand(1, 2, 128))   # one key: its value
