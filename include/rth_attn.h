@@ -365,7 +365,8 @@ int rth_attn_packed(uint16_t* out, const uint16_t* q, const uint16_t* k, const u
  * one row per sequence, row b of sequence b) to the sequences' pages: row t of
  * sequence b at position at_pos[b] + t - cu_seqlens[b] of it, byte for byte
  * as rth_kv_append_fp8_paged would. A row whose position lies outside the table, or
- * whose table entry names no page, is not stored. head_dim % 8 == 0, 8 <=
+ * whose table entry names no page, is not stored. Rows of one call go to positions of
+ * their own (sequences that share a page do not both write to it). head_dim % 8 == 0, 8 <=
  * head_dim <= 512. */
 int rth_kv_append_fp8_batch(uint8_t* k_cache, uint8_t* v_cache, float* k_scale, float* v_scale,
                             const uint16_t* k, const uint16_t* v, int64_t k_stride,

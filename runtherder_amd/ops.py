@@ -384,7 +384,7 @@ def kv_append_fp8_batch(k_cache, v_cache, k_scale, v_scale, k, v, at_pos, block_
     """Appends a batch's rows (k, v [rows, Hkv, D], packed by cu_seqlens, or
     one row per sequence) to the pages of their sequences, sequence b from
     position at_pos[b] on; bytes as PagedKVCache.append's. Rows without a page
-    are not stored."""
+    are not stored. Sequences that share a page do not both write to it."""
     blocks = _need_slabs_of(k_cache, v_cache, k_scale, v_scale, block_size, num_kv_heads,
                             head_dim, _current_device())
     _append_batch(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import runtherder_amd as R
-from batch_util import cu_of, ints, normal
+from batch_util import ints, normal
 from gpu_util import DEV, step, sync
 
 pytestmark = pytest.mark.gpu
@@ -35,7 +35,9 @@ def test_cache_past_4_gib():
     for c in (wide, small):
         step(f"append and decode in {c.num_blocks} pages")
         for layer in range(2):
-            c.append_batch(layer, k, v, ints([0, 0]), tables[c], ints(cu_of(lens)))
+            # (The first two pages, which both hold, are written by the second alone.)
+            c.append_batch(layer, k[700:], v[700:], ints([0]), tables[c][1:], ints([0, 1000]))
+            c.append_batch(layer, k[:188], v[:188], ints([512]), tables[c][:1], ints([0, 188]))
         for layer in range(2):
             for prefix in (None, tables[c][1]):
                 o = torch.empty((2, HKV, D), dtype=torch.bfloat16, device=DEV)
