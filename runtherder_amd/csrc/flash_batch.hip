@@ -19,9 +19,9 @@
 //  * Own keys (own_units, the other workgroups of the launch): the tiles of all
 //    sequences are dealt out in runs of equal length, so that long sequences
 //    spread over the chip and short ones do not wait for them; a wave per
-//    (run, kv head). The number of runs fits the scratch whatever the lengths,
+//    (run, kv head or two). The number of runs fits the scratch whatever the lengths,
 //    which live on the device.
-//  * A wave's tile: K and V codes and scales of 32 keys (64 at head_dim 64), one tile in
+//  * A wave's tile: K and V codes and scales of 32 keys (at head_dim 64 of two kv heads), one tile in
 //    registers ahead, through the wave's own LDS (no barriers): K rows are read
 //    back in the MFMA layout, V transposed by ds_read_b64_tr_b8. E4M3 codes are
 //    exact in bf16; the per-key scales are applied in fp32 to the scores and to
@@ -33,7 +33,7 @@
 // launches and the chain table -> page -> tile), 32 behind 8192 27 us (the same chain and
 // 21 MB), 128 behind 32768 105 us (69 GFLOP, 0.66 PFLOP/s; in the tile loop 0.99,
 // the rest is its start, the own keys and 35 MB of partials); 48 sequences of 100 to
-// 6000 own keys, head_dim 64, 35 us (bytes: 4.5 TB/s).
+// 6000 own keys, head_dim 64, 35 us (bytes: 4.4 TB/s).
 #include <algorithm>
 #include <type_traits>
 
@@ -108,6 +108,7 @@ __device__ __forceinline__ int wave_exclusive_i(int v, int lane, int& total) {
 // own keys: slots of runs.
 struct BatchPlan {
     int q_blocks;      // blocks of 16 q heads of a kv head
+    int head_units;    // kv heads, by the tiles of a wave
     int slots;
     int waves;         // of a workgroup
     int splits;        // of the prefix
@@ -130,25 +131,30 @@ __device__ __forceinline__ PrefixRuns prefix_runs(int tiles, const BatchPlan& p)
 
 // ---- a wave against tiles of its own ------------------------------------------
 
+// A wave's tile: 32 keys of a kv head, at head_dim 64 of two neighbours, so that
+// its loads take whole 128-byte lines (48 sequences of 100 to 6000 own keys, one head's
+// 64 keys -> two heads' 32: 45 -> 35 us).
 template <int D>
 struct WaveTile {
     static constexpr int kRowsQ  = 16;                    // query rows of a wave
-    static constexpr int kN      = D == 64 ? 64 : 32;     // keys
-    static constexpr int kSub    = kN / kHalf;
+    static constexpr int kN      = kHalf;                 // keys
+    static constexpr int kHeads  = D == 64 ? 2 : 1;
     static constexpr int kPitch  = D + 16;                // bytes per row in LDS
-    // V rows 16.. of a half lie this much further: the transposing reads take
+    // V rows 16.. lie this much further: the transposing reads take
     // rows 16 apart at once, which no pitch spreads over the banks.
     static constexpr int kSkew   = D == 64 ? 32 : D == 128 ? 16 : 64;
-    static constexpr int kVHalf  = kHalf * kPitch + kSkew;
-    static constexpr int kCpr    = D / 16;                // 16-byte chunks per row
-    static constexpr int kRows   = kWave / kCpr;          // rows of one load
+    static constexpr int kKHead  = kN * kPitch;           // a head's K, and V
+    static constexpr int kVHead  = kN * kPitch + kSkew;
+    static constexpr int kCpr    = D / 16;                // 16-byte chunks per row of a head
+    static constexpr int kLine   = kHeads * kCpr;         // of all heads
+    static constexpr int kRows   = kWave / kLine;         // keys of one load
     static constexpr int kLoads  = kN / kRows;
-    static constexpr int kV      = kN * kPitch;           // where V, and the factors start
-    static constexpr int kF      = kV + kSub * kVHalf;
-    static constexpr int kBytes  = kF + 2 * kN * 4;
+    static constexpr int kV      = kHeads * kKHead;       // where V, and the factors start
+    static constexpr int kF      = kV + kHeads * kVHead;
+    static constexpr int kBytes  = kF + 2 * kHeads * kN * 4;
     static constexpr int kArea   = kRowsQ * (D + 2);      // floats a wave hands over
     template <int kW>   // waves of a workgroup
-    static constexpr int kLds = std::max(kW * kBytes, kW / 2 * kArea * 4);
+    static constexpr int kLds = std::max(kW * kBytes, kW / 2 * kHeads * kArea * 4);
 };
 
 // 16 query rows (the columns of v_mfma_f32_16x16x32_bf16, lane l: row l % 16) of a
@@ -157,134 +163,138 @@ struct WaveTile {
 template <int D>
 struct WaveRows {
     using T = WaveTile<D>;
-    static constexpr int kKS = D / 32, kDB = D / 16;
+    static constexpr int kKS = D / 32, kDB = D / 16, kHeads = T::kHeads;
 
     const BatchView& t;
     uint8_t*         lds;   // the wave's
-    int              lane, kvh;
+    int              lane, kvh;   // kvh: the first of the tile's heads
+    int              heads;       // how many it has
     float            scale_log2;
-    bf16x8 qf[kKS];   // k-step 2 j + e of lane (row, g): d = 64 j + 16 g + 8 e .. + 7
-    f32x4  o[kDB];    // lane (row, g): d = 16 b + 4 g .. + 3
-    float  m_ref, l_run;
+    bf16x8 qf[kHeads][kKS];   // k-step 2 j + e of lane (row, g): d = 64 j + 16 g + 8 e .. + 7
+    f32x4  o[kHeads][kDB];    // lane (row, g): d = 16 b + 4 g .. + 3
+    float  m_ref[kHeads], l_run[kHeads];
     bool   start;
 
     u32x4 kreg[T::kLoads], vreg[T::kLoads];
-    float freg[T::kSub];
-    int   lo[T::kSub], hi[T::kSub];   // rows of the loaded halves that count
-    bool  there[T::kSub];
+    float freg[kHeads];
+    int   lo, hi;   // rows of the loaded tile that count
+    bool  there;
 
     __device__ __forceinline__ WaveRows(const BatchView& view, uint8_t* l, int ln, int kv, float sc)
-        : t(view), lds(l), lane(ln), kvh(kv), scale_log2(sc), m_ref(0.0f), l_run(0.0f), start(true) {
+        : t(view), lds(l), lane(ln), kvh(kv), heads(min(view.hkv - kv, kHeads)), scale_log2(sc),
+          start(true) {
 #pragma unroll
-        for (int b = 0; b < kDB; ++b) {
-            o[b] = f32x4{};
+        for (int u = 0; u < kHeads; ++u) {
+            m_ref[u] = 0.0f;
+            l_run[u] = 0.0f;
+#pragma unroll
+            for (int b = 0; b < kDB; ++b) {
+                o[u][b] = f32x4{};
+            }
         }
     }
 
-    __device__ __forceinline__ void load_q(const uint16_t* row) {
+    // row: the lane's row of the first head; `next`: as far as the next head's. (A head
+    // that is not there gets the first one's.)
+    __device__ __forceinline__ void load_q(const uint16_t* row, int next) {
         const int g = lane >> 4;
 #pragma unroll
-        for (int s = 0; s < kKS; ++s) {
-            qf[s] = *reinterpret_cast<const bf16x8*>(row + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
-        }
-    }
-
-    // The table entries of tile i (one per half), in every lane.
-    __device__ __forceinline__ void entries(const int* table, int i, int to, int (&e)[T::kSub]) const {
+        for (int u = 0; u < kHeads; ++u) {
+            const uint16_t* x = row + (u < heads ? u * next : 0);
 #pragma unroll
-        for (int u = 0; u < T::kSub; ++u) {
-            const int key = i * T::kN + u * kHalf;
-            e[u]          = key < to ? table[key >> t.block_shift] : -1;
+            for (int s = 0; s < kKS; ++s) {
+                qf[u][s] = *reinterpret_cast<const bf16x8*>(x + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
+            }
         }
     }
 
-    // Codes are read once (nontemporal) where a head's row is a whole 128-byte line;
-    // the heads' waves of a workgroup share the lines of shorter rows.
+    // The table entry of tile i, in every lane.
+    __device__ __forceinline__ int entry(const int* table, int i, int to) const {
+        const int key = i * T::kN;
+        return key < to ? table[key >> t.block_shift] : -1;
+    }
+
+    // Codes are read once (nontemporal).
     static __device__ __forceinline__ u32x4 codes(const uint8_t* p, uint32_t off) {
-        if constexpr (D >= 128) {
-            return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + off));
-        } else {
-            return *reinterpret_cast<const u32x4*>(p + off);
-        }
+        return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + off));
     }
 
-    // Loads tile i. Rows outside [from, to) repeat one inside (their V is made
+    // Loads tile i, on page e. Rows outside [from, to) repeat one inside (their V is made
     // zeros as it is staged, and their factors are).
-    __device__ __forceinline__ void load(int i, const Keys& keys, const int (&e)[T::kSub]) {
+    __device__ __forceinline__ void load(int i, const Keys& keys, int e) {
         const int ln = again(lane);   // (addresses: computed anew for each tile)
         const uint32_t stride = static_cast<uint32_t>(t.hkv) * D;
-        const uint32_t r0 = static_cast<uint32_t>(ln / T::kCpr), chunk = static_cast<uint32_t>(ln % T::kCpr);
-        constexpr int  kPer = kHalf / T::kRows;   // loads of a half
+        const uint32_t r0 = static_cast<uint32_t>(ln / T::kLine);
+        const uint32_t chunk = static_cast<uint32_t>(ln % (heads < kHeads ? T::kCpr : T::kLine));
+        const int page = uniform(e), key0 = i * T::kN;
+        lo    = max(keys.from - key0, 0);
+        hi    = min(keys.to - key0, T::kN);
+        there = t.is_page(page) && lo < hi;
+        if (!there) {   // (the first page's rows, which nothing uses)
+            lo = 0;
+            hi = T::kN;
+        }
+        const int64_t  row = t.row(there ? page : 0, key0);
+        const int64_t  at  = row * stride + static_cast<int64_t>(kvh) * D;
+        const uint8_t* kp  = t.k + at;
+        const uint8_t* vp  = t.v + at;
+        if (lo == 0 && hi == T::kN) {
+            const uint32_t off = r0 * stride + 16u * chunk;
 #pragma unroll
-        for (int u = 0; u < T::kSub; ++u) {
-            const int page = uniform(e[u]), key0 = i * T::kN + u * kHalf;
-            lo[u]    = max(keys.from - key0, 0);
-            hi[u]    = min(keys.to - key0, kHalf);
-            there[u] = t.is_page(page) && lo[u] < hi[u];
-            if (!there[u]) {   // (the first page's rows, which nothing uses)
-                lo[u] = 0;
-                hi[u] = kHalf;
+            for (int s = 0; s < T::kLoads; ++s) {
+                const uint32_t more = static_cast<uint32_t>(s * T::kRows) * stride;
+                kreg[s] = codes(kp + more, off);
+                vreg[s] = codes(vp + more, off);
             }
-            const int64_t  row = t.row(there[u] ? page : 0, key0);
-            const int64_t  at  = row * stride + static_cast<int64_t>(kvh) * D;
-            const uint8_t* kp  = t.k + at;
-            const uint8_t* vp  = t.v + at;
-            if (lo[u] == 0 && hi[u] == kHalf) {
-                const uint32_t off = r0 * stride + 16u * chunk;
+        } else {
 #pragma unroll
-                for (int s = 0; s < kPer; ++s) {
-                    const uint32_t more = static_cast<uint32_t>(s * T::kRows) * stride;
-                    kreg[u * kPer + s] = codes(kp + more, off);
-                    vreg[u * kPer + s] = codes(vp + more, off);
-                }
-            } else {
-#pragma unroll
-                for (int s = 0; s < kPer; ++s) {
-                    const int      r   = min(max(s * T::kRows + static_cast<int>(r0), lo[u]), hi[u] - 1);
-                    const uint32_t off = static_cast<uint32_t>(r) * stride + 16u * chunk;
-                    kreg[u * kPer + s] = codes(kp, off);
-                    vreg[u * kPer + s] = codes(vp, off);
-                }
+            for (int s = 0; s < T::kLoads; ++s) {
+                const int      r   = min(max(s * T::kRows + static_cast<int>(r0), lo), hi - 1);
+                const uint32_t off = static_cast<uint32_t>(r) * stride + 16u * chunk;
+                kreg[s] = codes(kp, off);
+                vreg[s] = codes(vp, off);
             }
-            // Factors: lanes 0..31 of K, the others of V.
-            const int    r = ln & 31;
-            const float* f = (ln < 32 ? t.ks : t.vs) + row * t.hkv + kvh;
-            freg[u] = f[static_cast<uint32_t>(min(max(r, lo[u]), hi[u] - 1)) * static_cast<uint32_t>(t.hkv)];
+        }
+        // Factors: lanes 0..31 of K, the others of V.
+        const float* f = (ln < 32 ? t.ks : t.vs) + row * t.hkv + kvh +
+                         static_cast<uint32_t>(min(max(ln & 31, lo), hi - 1)) * static_cast<uint32_t>(t.hkv);
+#pragma unroll
+        for (int u = 0; u < kHeads; ++u) {
+            freg[u] = f[u < heads ? u : 0];
         }
     }
 
     __device__ __forceinline__ void stage() {
         const int ln = again(lane);
-        const int r0 = ln / T::kCpr, chunk = ln % T::kCpr;
-        constexpr int kPer = kHalf / T::kRows;
-        float* f = reinterpret_cast<float*>(lds + T::kF);
+        const int r0 = ln / T::kLine, head = ln % T::kLine / T::kCpr, chunk = ln % T::kCpr;
+        float*     f    = reinterpret_cast<float*>(lds + T::kF);
+        const bool edge = lo > 0 || hi < T::kN;
+        uint8_t*   at   = lds + r0 * T::kPitch + 16 * chunk;
 #pragma unroll
-        for (int u = 0; u < T::kSub; ++u) {
-            const bool edge = lo[u] > 0 || hi[u] < kHalf;
-            uint8_t*   at   = lds + r0 * T::kPitch + 16 * chunk;
-#pragma unroll
-            for (int s = 0; s < kPer; ++s) {
-                const int r = s * T::kRows;
-                u32x4     v = vreg[u * kPer + s];
-                if (edge && (r + r0 < lo[u] || r + r0 >= hi[u])) {
-                    v = u32x4{};
-                }
-                *reinterpret_cast<u32x4*>(at + (u * kHalf + r) * T::kPitch) = kreg[u * kPer + s];
-                *reinterpret_cast<u32x4*>(at + T::kV + u * T::kVHalf + r * T::kPitch + (r >= 16 ? T::kSkew : 0)) = v;
+        for (int s = 0; s < T::kLoads; ++s) {
+            const int r = s * T::kRows;
+            u32x4     v = vreg[s];
+            if (edge && (r + r0 < lo || r + r0 >= hi)) {
+                v = u32x4{};
             }
-            const int  r  = ln & 31;
-            const bool in = r >= lo[u] && r < hi[u];
-            f[(ln < 32 ? 0 : T::kN) + u * kHalf + r] = in ? freg[u] * (ln < 32 ? scale_log2 : 1.0f) : 0.0f;
+            *reinterpret_cast<u32x4*>(at + head * T::kKHead + r * T::kPitch) = kreg[s];
+            *reinterpret_cast<u32x4*>(at + T::kV + head * T::kVHead + r * T::kPitch + (r >= 16 ? T::kSkew : 0)) = v;
+        }
+        const int  r  = ln & 31;
+        const bool in = r >= lo && r < hi;
+#pragma unroll
+        for (int u = 0; u < kHeads; ++u) {
+            f[(ln < 32 ? 0 : kHeads * T::kN) + u * T::kN + r] = in ? freg[u] * (ln < 32 ? scale_log2 : 1.0f) : 0.0f;
         }
     }
 
-    // The staged keys u * 32 .. + 31, of which this lane's row sees rows lo .. hi - 1.
-    __device__ __forceinline__ void half(int u, int lo, int hi) {
+    // The staged keys of head u, of which this lane's row sees rows lo .. hi - 1.
+    __device__ __forceinline__ void keys_of(int u, int lo, int hi) {
         const int      ln = again(lane), row = ln & 15, g = ln >> 4;
-        const uint8_t* lk = lds + u * kHalf * T::kPitch;
-        const uint8_t* lv = lds + T::kV + u * T::kVHalf;
-        const float*   ls = reinterpret_cast<const float*>(lds + T::kF) + u * kHalf;
-        // Register 4 a + e of a lane: key 16 a + 4 g + e of the half.
+        const uint8_t* lk = lds + u * T::kKHead;
+        const uint8_t* lv = lds + T::kV + u * T::kVHead;
+        const float*   ls = reinterpret_cast<const float*>(lds + T::kF) + u * T::kN;
+        // Register 4 a + e of a lane: key 16 a + 4 g + e of the tile.
         float s[8];
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
@@ -295,16 +305,16 @@ struct WaveRows {
                 const u32x4 w = *reinterpret_cast<const u32x4*>(lk + (16 * a + row) * T::kPitch + 64 * j + 16 * g);
                 bf16x8 a0, a1;
                 e4m3x16_to_bf16x8x2(w, a0, a1);
-                x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, qf[2 * j], x, 0, 0, 0);
-                x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, qf[2 * j + 1], x, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, qf[u][2 * j], x, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, qf[u][2 * j + 1], x, 0, 0, 0);
             }
             const f32x4 kf = *reinterpret_cast<const f32x4*>(ls + 16 * a + 4 * g);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                s[4 * a + e] = fmaf(x[e], kf[e], -m_ref);
+                s[4 * a + e] = fmaf(x[e], kf[e], -m_ref[u]);
             }
         }
-        if (__any(lo > 0 || hi < kHalf)) {
+        if (__any(lo > 0 || hi < T::kN)) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int r = 16 * (e >> 2) + 4 * g + (e & 3);
@@ -318,7 +328,7 @@ struct WaveRows {
             sum = 0.0f;
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
-                const f32x4 vf = *reinterpret_cast<const f32x4*>(ls + T::kN + 16 * a + 4 * g);
+                const f32x4 vf = *reinterpret_cast<const f32x4*>(ls + kHeads * T::kN + 16 * a + 4 * g);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float x = __builtin_amdgcn_exp2f(s[4 * a + e]);
@@ -340,20 +350,19 @@ struct WaveRows {
             const bool  need  = wave_xor_max(wave_xor_max(high ? 1.0f : 0.0f, 16), 32) != 0.0f;
             const float up    = start ? (top == -INFINITY ? 0.0f : top) : need ? fmaxf(top, 0.0f) : 0.0f;
             const float alpha = start ? 1.0f : __builtin_amdgcn_exp2f(-up);
-            m_ref += up;
-            l_run *= alpha;
+            m_ref[u] += up;
+            l_run[u] *= alpha;
 #pragma unroll
             for (int b = 0; b < kDB; ++b) {
-                o[b] *= alpha;
+                o[u][b] *= alpha;
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 s[e] -= up;
             }
             weights();
-            start = false;
         }
-        l_run += sum;
+        l_run[u] += sum;
         pin();
         // V^T: lane (d, g), the keys of p: 4 g + 0..3 and 16 + 4 g + 0..3. A group of
         // 16 lanes reads eight keys' 16 d and gets them transposed: ln i points at
@@ -367,7 +376,7 @@ struct WaveRows {
         for (int b = 0; b < kDB; ++b) {
             const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((LdsPtr)const_cast<uint8_t*>(vp + 16 * b));
             const u32x2 x = {static_cast<uint32_t>(w.x), static_cast<uint32_t>(w.y)};
-            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e4m3x8_to_bf16x8(x), p, o[b], 0, 0, 0);
+            o[u][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e4m3x8_to_bf16x8(x), p, o[u][b], 0, 0, 0);
             if (b % 4 == 3) {
                 pin();
             }
@@ -381,30 +390,28 @@ struct WaveRows {
         if (first >= last) {
             return;
         }
-        int e[T::kSub], next[T::kSub];
-        entries(table, first, keys.to, e);
-        entries(table, first + step, first + step < last ? keys.to : 0, next);
+        int e = entry(table, first, keys.to);
+        int next = entry(table, first + step, first + step < last ? keys.to : 0);
         load(first, keys, e);
         for (int i = first; i < last; i += step) {
-            bool is[T::kSub];
-#pragma unroll
-            for (int u = 0; u < T::kSub; ++u) {
-                is[u] = there[u];
-                e[u]  = next[u];
-            }
+            const bool is = there;
+            e             = next;
             stage();
             if (i + 2 * step < last) {
-                entries(table, i + 2 * step, keys.to, next);
+                next = entry(table, i + 2 * step, keys.to);
             }
             if (i + step < last) {
                 load(i + step, keys, e);
             }
+            if (is) {
+                const int key0 = i * T::kN;
 #pragma unroll
-            for (int u = 0; u < T::kSub; ++u) {
-                const int key0 = i * T::kN + u * kHalf;
-                if (is[u]) {
-                    half(u, keys.from - key0, min(keys.to, end) - key0);
+                for (int u = 0; u < kHeads; ++u) {
+                    if (u < heads) {
+                        keys_of(u, keys.from - key0, min(keys.to, end) - key0);
+                    }
                 }
+                start = false;
             }
         }
     }
@@ -413,9 +420,9 @@ struct WaveRows {
         return wave_xor_sum(wave_xor_sum(x, 16), 32);
     }
 
-    // m, l (summed over the row's lanes) and O of this lane's row, as one of
+    // m, l (summed over the row's lanes) and O of this lane's row of head u, as one of
     // `rows` partials at `part`.
-    __device__ __forceinline__ void write(float* part, int64_t rows, int64_t row, float m, float l) const {
+    __device__ __forceinline__ void write(int u, float* part, int64_t rows, int64_t row, float m, float l) const {
         const int g = lane >> 4;
         if (g == 0) {
             part[row]        = m;
@@ -424,43 +431,47 @@ struct WaveRows {
         float* po = part + 2 * rows + row * D + 4 * g;
 #pragma unroll
         for (int b = 0; b < kDB; ++b) {
-            *reinterpret_cast<f32x4_a4*>(po + 16 * b) = o[b];
+            *reinterpret_cast<f32x4_a4*>(po + 16 * b) = o[u][b];
         }
     }
 
     // Joins the results of the workgroup's waves into wave 0's, by halves: the
     // upper half of the waves left hands over through LDS. m and l: as write().
     template <int kW>
-    __device__ __forceinline__ void join(float* all, int wave, float& m, float& l) {
+    __device__ __forceinline__ void join(float* all, int wave, float (&m)[kHeads], float (&l)[kHeads]) {
 #pragma unroll
         for (int n = kW / 2; n > 0; n >>= 1) {
             __syncthreads();   // tiles, or the step before, are done with
-            // A wave's area: [D / 16][64 lanes] quads of O, then m and l of 16 rows.
-            float* a = all + (wave % n) * T::kArea;
+            // A wave's area, for each head: [D / 16][64 lanes] quads of O, then m and l of 16 rows.
+            float* a = all + (wave % n) * kHeads * T::kArea;
             if (wave >= n && wave < 2 * n) {
 #pragma unroll
-                for (int b = 0; b < kDB; ++b) {
-                    *reinterpret_cast<f32x4*>(a + (b * kWave + lane) * 4) = o[b];
-                }
-                if (lane < 16) {
-                    a[16 * D + lane]      = m;
-                    a[16 * D + 16 + lane] = l;
+                for (int u = 0; u < kHeads; ++u) {
+#pragma unroll
+                    for (int b = 0; b < kDB; ++b) {
+                        *reinterpret_cast<f32x4*>(a + u * T::kArea + (b * kWave + lane) * 4) = o[u][b];
+                    }
+                    if (lane < 16) {
+                        a[u * T::kArea + 16 * D + lane]      = m[u];
+                        a[u * T::kArea + 16 * D + 16 + lane] = l[u];
+                    }
                 }
             }
             __syncthreads();
             if (wave < n) {
-                const float m1 = a[16 * D + (lane & 15)], l1 = a[16 * D + 16 + (lane & 15)];
-                const float top = m1 != m1 ? m1 : fmaxf(m, m1);
-                const float f0 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-                const float f1 = m1 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m1 - top);
-                l = f0 * l + f1 * l1;
-                m = top;
 #pragma unroll
-                for (int b = 0; b < kDB; ++b) {
-                    const f32x4 x = *reinterpret_cast<const f32x4*>(a + (b * kWave + lane) * 4);
+                for (int u = 0; u < kHeads; ++u) {
+                    const float* x  = a + u * T::kArea;
+                    const float  m1 = x[16 * D + (lane & 15)], l1 = x[16 * D + 16 + (lane & 15)];
+                    const float top = m1 != m1 ? m1 : fmaxf(m[u], m1);
+                    const float f0 = m[u] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[u] - top);
+                    const float f1 = m1 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m1 - top);
+                    l[u] = f0 * l[u] + f1 * l1;
+                    m[u] = top;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        o[b][i] = f0 * o[b][i] + f1 * x[i];
+                    for (int b = 0; b < kDB; ++b) {
+                        const f32x4 y = *reinterpret_cast<const f32x4*>(x + (b * kWave + lane) * 4);
+                        o[u][b] = f0 * o[u][b] + f1 * y;
                     }
                 }
             }
@@ -481,7 +492,7 @@ __device__ __forceinline__ void prefix_units(uint8_t* lds, int bid, int prefix,
     const int hq   = t.hkv * t.group;
     const int tiles = (prefix + T::kN - 1) / T::kN;
     const PrefixRuns runs = prefix_runs(tiles, bp);
-    const int at = uniform(bid / t.hkv), kvh = bid - at * t.hkv;
+    const int at = uniform(bid / bp.head_units), kvh = (bid - at * bp.head_units) * T::kHeads;
     const int split = uniform(at / bp.row_blocks), rb = at - split * bp.row_blocks;
     if (split >= runs.live) {
         return;
@@ -490,19 +501,28 @@ __device__ __forceinline__ void prefix_units(uint8_t* lds, int bid, int prefix,
     const int row  = min(rb * 16 + col, rows - 1);
     const int b = row / t.group, head = kvh * t.group + (row - b * t.group);
     WaveRows<D> w(t, lds + wave * T::kBytes, lane, kvh, scale_log2);
-    w.load_q(q + b * q_stride + static_cast<int64_t>(head) * D);
+    w.load_q(q + b * q_stride + static_cast<int64_t>(head) * D, t.group * D);
     const int first = split * runs.per;
     w.run(t.prefix_table, Keys{0, prefix}, first + wave, min(first + runs.per, tiles), kW,
           t.lens[b]);
-    float l = w.row_sum(w.l_run), m = l == 0.0f ? -INFINITY : w.m_ref;
+    const int64_t all = static_cast<int64_t>(bp.splits) * t.num_seqs * hq;
+    float m[T::kHeads], l[T::kHeads];
+#pragma unroll
+    for (int u = 0; u < T::kHeads; ++u) {
+        l[u] = w.row_sum(w.l_run[u]);
+        m[u] = l[u] == 0.0f ? -INFINITY : w.m_ref[u];
+    }
     w.template join<kW>(reinterpret_cast<float*>(lds), wave, m, l);
-    if (wave == 0 && rb * 16 + col < rows) {
-        const int64_t all = static_cast<int64_t>(bp.splits) * t.num_seqs * hq;
-        w.write(shared, all, (static_cast<int64_t>(split) * t.num_seqs + b) * hq + head, m, l);
+#pragma unroll
+    for (int u = 0; u < T::kHeads; ++u) {
+        if (wave == 0 && rb * 16 + col < rows && u < w.heads) {
+            w.write(u, shared, all, (static_cast<int64_t>(split) * t.num_seqs + b) * hq + head + u * t.group, m[u],
+                    l[u]);
+        }
     }
 }
 
-// Workgroup `bid` of the own keys: (slot, group of kW (kv head, block of 16 q heads) units).
+// Workgroup `bid` of the own keys: (slot, group of kW units: the kv heads of a tile, block of 16 q heads of each).
 template <int D, int kW>
 __device__ __forceinline__ void own_units(uint8_t* lds, int bid, int prefix,
                                           const uint16_t* __restrict__ q, int64_t q_stride,
@@ -513,13 +533,12 @@ __device__ __forceinline__ void own_units(uint8_t* lds, int bid, int prefix,
     const int tid  = static_cast<int>(threadIdx.x);
     const int wave = uniform(tid / kWave), lane = tid & (kWave - 1), col = lane & 15;
     const int hq   = t.hkv * t.group;
-    const int units  = t.hkv * bp.q_blocks;
-    const int groups = (units + kW - 1) / kW;
-    const int slot = uniform(bid / groups), unit = (bid - slot * groups) * kW + wave;
-    if (unit >= units) {
+    const int units  = bp.head_units * bp.q_blocks;
+    const int slot = uniform((bid * kW + wave) / units), unit = bid * kW + wave - slot * units;
+    if (slot >= bp.slots) {
         return;
     }
-    const int kvh = uniform(unit / bp.q_blocks), qb = unit - kvh * bp.q_blocks;
+    const int of = uniform(unit / bp.q_blocks), qb = unit - of * bp.q_blocks, kvh = of * T::kHeads;
 
     // Which run of which sequence this slot is. Slot 0 writes the plan down.
     int total = 0;
@@ -559,12 +578,15 @@ __device__ __forceinline__ void own_units(uint8_t* lds, int bid, int prefix,
     const int t1 = min(t0 + per, (keys.to - 1) / T::kN + 1);
     const int head = kvh * t.group + min(qb * 16 + col, t.group - 1);
     WaveRows<D> w(t, lds + wave * T::kBytes, lane, kvh, scale_log2);
-    w.load_q(q + seq * q_stride + static_cast<int64_t>(head) * D);
+    w.load_q(q + seq * q_stride + static_cast<int64_t>(head) * D, t.group * D);
     w.run(t.tables + static_cast<int64_t>(seq) * t.table_blocks, keys, t0, t1, 1, keys.to);
-    const float l = w.row_sum(w.l_run);
-    if (qb * 16 + col < t.group) {
-        w.write(own, static_cast<int64_t>(bp.slots) * hq, static_cast<int64_t>(slot) * hq + head,
-                l == 0.0f ? -INFINITY : w.m_ref, l);
+#pragma unroll
+    for (int u = 0; u < T::kHeads; ++u) {
+        const float l = w.row_sum(w.l_run[u]);
+        if (qb * 16 + col < t.group && u < w.heads) {
+            w.write(u, own, static_cast<int64_t>(bp.slots) * hq,
+                    static_cast<int64_t>(slot) * hq + head + u * t.group, l == 0.0f ? -INFINITY : w.m_ref[u], l);
+        }
     }
 }
 
@@ -986,6 +1008,7 @@ BatchPlan batch_plan(int num_seqs, int hq, int hkv, int head_dim, int cus, bool 
     const int group = hq / hkv, rows = num_seqs * group;
     BatchPlan p;
     p.q_blocks   = (group + 15) / 16;
+    p.head_units = head_dim == 64 ? (hkv + 1) / 2 : hkv;
     p.tile_waves = !shared || rows <= 64 ? 0 : head_dim < 256 && rows > 128 ? 8 : 4;
     const int per_block = p.tile_waves == 0 ? 16 : 32 * p.tile_waves;
     p.row_blocks = (rows + per_block - 1) / per_block;
@@ -1000,11 +1023,11 @@ BatchPlan batch_plan(int num_seqs, int hq, int hkv, int head_dim, int cus, bool 
     // head_dim 256, two per compute unit), half of it the prefix's; prefix tiles
     // take up to one round of their own, one workgroup per compute unit.
     const int round  = cus * (p.tile_waves != 0 ? 1 : head_dim == 256 ? 2 : 3);
-    const int wgs    = p.row_blocks * hkv, most = p.tile_waves == 0 ? round / 2 : round;
+    const int wgs  = p.row_blocks * (p.tile_waves == 0 ? p.head_units : hkv);
+    const int most = p.tile_waves == 0 ? round / 2 : round;
     p.splits         = shared ? std::max(1, std::min(256, most / wgs)) : 0;
     const int left   = shared && p.tile_waves == 0 ? std::max(round - wgs * p.splits, round / 4) : round;
-    const int groups = (hkv * p.q_blocks + p.waves - 1) / p.waves;   // workgroups of a slot
-    p.slots = std::max(left / groups, num_seqs + std::max(8, num_seqs / 4));
+    p.slots = std::max(left * p.waves / (p.head_units * p.q_blocks), num_seqs + std::max(8, num_seqs / 4));
     return p;
 }
 
@@ -1019,8 +1042,8 @@ hipError_t launch_batch(uint16_t* out, int64_t out_stride, const uint16_t* q, in
     int*        plan       = reinterpret_cast<int*>(partial);
     float*      own        = partial + plan_floats(t.num_seqs);
     float*      shared     = own + static_cast<std::size_t>(p.slots) * hq * (D + 2);
-    const int   pre        = p.row_blocks * t.hkv * p.splits;
-    const dim3  grid(static_cast<unsigned>(pre + p.slots * ((t.hkv * p.q_blocks + p.waves - 1) / p.waves)));
+    const int   pre        = p.row_blocks * (p.tile_waves == 0 ? p.head_units : t.hkv) * p.splits;
+    const dim3  grid(static_cast<unsigned>(pre + (p.slots * p.head_units * p.q_blocks + p.waves - 1) / p.waves));
     const dim3  block(static_cast<unsigned>(p.waves * kWave));
 #define RTH_BATCH(W, G)                                                                        \
     batch_kernel<D, W, G><<<grid, block, 0, stream>>>(q, q_stride, t, own, plan, shared, p, pre, \
