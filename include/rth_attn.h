@@ -341,8 +341,8 @@ int rth_rmsnorm_lanes(int hidden_dim);
  *
  * Packed rows: the tokens of num_seqs sequences one behind the other; sequence
  * b holds rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (cu_seqlens: num_seqs + 1
- * device ints, ascending; bounds past num_rows are taken as num_rows). Rows
- * behind the last sequence are neither read nor written. Row strides are in
+ * device ints, ascending; bounds past num_rows are taken as num_rows). What rows
+ * behind the last sequence hold does not matter, and they are not written. Row strides are in
  * elements, multiples of 8, at least heads * head_dim and at most 2^24 (so q, k
  * and v may be slices of one projection's rows). Rows of q, k, v and out start 16-byte aligned.
  *
@@ -385,7 +385,8 @@ int rth_kv_append_fp8_batch(uint8_t* k_cache, uint8_t* v_cache, float* k_scale, 
  * an unused slot, its output row is zeros. A sequence shorter than the prefix sees
  * its lens[b] keys of it (where the others are finite: the rows of a kv head are one
  * product, in which a NaN or an infinity times a weight of 0 is a NaN). Keys past a table's end, and keys whose
- * table entry names no page, are left out. head_dim 64, 128, 256; any Hq / Hkv.
+ * table entry names no page, are left out. head_dim 64, 128, 256; any Hq / Hkv;
+ * num_seqs * Hq <= 2^24, num_seqs * table_blocks * block_size <= 2^35.
  * partial: rth_batch_scratch_floats floats, 16-byte aligned, no
  * initialization needed, not shared by calls that overlap (graphs included). */
 size_t rth_batch_scratch_floats(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim);

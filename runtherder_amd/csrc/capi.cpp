@@ -919,6 +919,9 @@ int rth_attn_decode_batch(uint16_t* out, int64_t out_stride, const uint16_t* q, 
     if (int rc = check_tables(block_tables, table_blocks, num_blocks, block_size)) {
         return rc;
     }
+    // (Tiles of 32 keys of all sequences are counted in 32 bits.)
+    RTH_REQUIRE(static_cast<int64_t>(num_seqs) * table_blocks <= (int64_t{1} << 35) / block_size,
+                "num_seqs * table_blocks * block_size must be at most 2^35");
     return check_hip(rth::flash_batch_launch(out, out_stride, q, q_stride, k, v, k_scale, v_scale,
                                              block_tables, table_blocks, num_blocks,
                                              block_shift_of(block_size), lens, prefix_table,

@@ -86,12 +86,6 @@ __device__ __forceinline__ Keys own_keys(const BatchView& t, int b, int prefix) 
     return {prefix, static_cast<int>(min(static_cast<int64_t>(t.lens[b]), room))};
 }
 
-// Tiles per run such that all sequences' runs of that many tiles (the last one
-// of each shorter) fit in num_slots slots.
-__device__ __forceinline__ int tiles_per_slot(int total_tiles, int num_seqs, int num_slots) {
-    return max(1, (total_tiles + num_slots - num_seqs - 1) / (num_slots - num_seqs));
-}
-
 // Exclusive prefix sum over the wave's lanes, and the total.
 __device__ __forceinline__ int wave_exclusive_i(int v, int lane, int& total) {
     int x = v;
@@ -102,6 +96,36 @@ __device__ __forceinline__ int wave_exclusive_i(int v, int lane, int& total) {
     }
     total = __shfl(x, kWave - 1, kWave);
     return x - v;
+}
+
+// Tiles per run such that all sequences' runs of that many tiles (the last one
+// of each shorter) fit in num_slots slots: the fewest, by bisection, for up to
+// kChunks waves of sequences (tiles[c]: of sequence 64 c + lane), else as many as
+// always do (128 sequences of 1000 to 4000 keys, 155 -> 123 us).
+template <int kChunks>
+__device__ __forceinline__ int tiles_per_slot(int total_tiles, const int (&tiles)[kChunks], int num_seqs,
+                                              int num_slots) {
+    int hi = max(1, (total_tiles + num_slots - num_seqs - 1) / (num_slots - num_seqs));
+    if (num_seqs > kChunks * kWave) {
+        return hi;
+    }
+    int lo = max(1, (total_tiles + num_slots - 1) / num_slots);
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        int       runs = 0;
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+            if (c * kWave < num_seqs) {
+                runs += (tiles[c] + mid - 1) / mid;
+            }
+        }
+        if (uniform(wave_sum_i(runs)) <= num_slots) {
+            hi = mid;
+        } else {
+            lo = mid + 1;
+        }
+    }
+    return hi;
 }
 
 // How a launch is split. Prefix: splits of the keys for each block of rows;
@@ -541,12 +565,20 @@ __device__ __forceinline__ void own_units(uint8_t* lds, int bid, int prefix,
     const int of = uniform(unit / bp.q_blocks), qb = unit - of * bp.q_blocks, kvh = of * T::kHeads;
 
     // Which run of which sequence this slot is. Slot 0 writes the plan down.
-    int total = 0;
-    for (int b0 = 0; b0 < t.num_seqs; b0 += kWave) {
-        const int b = b0 + lane;
-        total += wave_sum_i(b < t.num_seqs ? own_keys(t, b, prefix).tiles(T::kN) : 0);
+    constexpr int kChunks = 4;
+    int           tiles[kChunks] = {}, total = 0;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        const int b = c * kWave + lane;
+        tiles[c]    = b < t.num_seqs ? own_keys(t, b, prefix).tiles(T::kN) : 0;
+        total += tiles[c];
     }
-    const int per = tiles_per_slot(total, t.num_seqs, bp.slots);
+    for (int b0 = kChunks * kWave; b0 < t.num_seqs; b0 += kWave) {
+        const int b = b0 + lane;
+        total += b < t.num_seqs ? own_keys(t, b, prefix).tiles(T::kN) : 0;
+    }
+    total         = uniform(wave_sum_i(total));
+    const int per = tiles_per_slot(total, tiles, t.num_seqs, bp.slots);
     int seq = -1, run = 0, base = 0;
     for (int b0 = 0; b0 < t.num_seqs; b0 += kWave) {
         const int b    = b0 + lane;
@@ -873,11 +905,17 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D> (&sm)[kG], int bid, in
 }
 
 // Workgroups: first the prefix's, then those of the own keys. kG > 0: the prefix by
-// prefix_tiles, two waves per SIMD (head_dim 256: one); kG == 0: by prefix_units,
-// three (two).
+// prefix_tiles, two waves per SIMD (head_dim 256: one); kG == 0 and four waves: by
+// prefix_units, three (two); kG == 0 and eight waves: there is none, and workgroups of
+// eight waves take all heads of a run together where there are as many (48 sequences of 100
+// to 6000 keys, one workgroup of eight per compute unit against three of four: 60 -> 54
+// us; two tiles ahead instead of one: 54 -> 56).
 constexpr int batch_waves(int w, int g) { return w * (g > 0 ? g : 1); }
+constexpr int batch_per_simd(int d, int w, int g) {
+    return g > 0 ? (d < 256 ? 2 : 1) : w == 8 ? 2 : d < 256 ? 3 : 2;
+}
 template <int D, int kW, int kG>
-__global__ __launch_bounds__(batch_waves(kW, kG) * kWave, (D < 256 ? 2 : 1) + (kG > 0 ? 0 : 1)) void batch_kernel(
+__global__ __launch_bounds__(batch_waves(kW, kG) * kWave, batch_per_simd(D, kW, kG)) void batch_kernel(
     const uint16_t* __restrict__ q, int64_t q_stride, BatchView t, float* __restrict__ own,
     int* __restrict__ plan, float* __restrict__ shared, BatchPlan bp, int prefix_wgs,
     float scale_log2) {
@@ -890,15 +928,17 @@ __global__ __launch_bounds__(batch_waves(kW, kG) * kWave, (D < 256 ? 2 : 1) + (k
     uint8_t*  units  = reinterpret_cast<uint8_t*>(&lds);
     const int bid    = static_cast<int>(blockIdx.x);
     const int prefix = prefix_keys(t);
-    if (bid < prefix_wgs) {
-        if constexpr (kG > 0) {
-            prefix_tiles<D, kW, kG>(lds.tiles, bid, prefix, q, q_stride, t, shared, bp, scale_log2);
-        } else {
-            prefix_units<D, kWaves>(units, bid, prefix, q, q_stride, t, shared, bp, scale_log2);
+    if constexpr (kG > 0 || kW == 4) {
+        if (bid < prefix_wgs) {
+            if constexpr (kG > 0) {
+                prefix_tiles<D, kW, kG>(lds.tiles, bid, prefix, q, q_stride, t, shared, bp, scale_log2);
+            } else {
+                prefix_units<D, kWaves>(units, bid, prefix, q, q_stride, t, shared, bp, scale_log2);
+            }
+            return;
         }
-    } else {
-        own_units<D, kWaves>(units, bid - prefix_wgs, prefix, q, q_stride, t, own, plan, bp, scale_log2);
     }
+    own_units<D, kWaves>(units, bid - prefix_wgs, prefix, q, q_stride, t, own, plan, bp, scale_log2);
 }
 
 // ---- joining a row's partials ------------------------------------------------------
@@ -1012,7 +1052,7 @@ BatchPlan batch_plan(int num_seqs, int hq, int hkv, int head_dim, int cus, bool 
     p.tile_waves = !shared || rows <= 64 ? 0 : head_dim < 256 && rows > 128 ? 8 : 4;
     const int per_block = p.tile_waves == 0 ? 16 : 32 * p.tile_waves;
     p.row_blocks = (rows + per_block - 1) / per_block;
-    p.waves = p.tile_waves == 0 || head_dim == 256 ? 4 : 8;
+    p.waves = head_dim == 256 || (p.tile_waves == 0 && shared) ? 4 : 8;
     // A tile per group of waves for short prefixes (32 sequences after 1000 keys, tiles
     // of a split 8 -> 2: 23 -> 17 us), eight before more than half the splits write partials
     // (64 after 8192, 4 -> 8: 39 -> 34; head_dim 256, whose tiles take twice as
@@ -1022,7 +1062,7 @@ BatchPlan batch_plan(int num_seqs, int hq, int hkv, int head_dim, int cus, bool 
     // Rounds of the chip's workgroups: one for a launch of units (three or, at
     // head_dim 256, two per compute unit), half of it the prefix's; prefix tiles
     // take up to one round of their own, one workgroup per compute unit.
-    const int round  = cus * (p.tile_waves != 0 ? 1 : head_dim == 256 ? 2 : 3);
+    const int round = cus * (p.tile_waves != 0 || p.waves == 8 ? 1 : head_dim == 256 ? 2 : 3);
     const int wgs  = p.row_blocks * (p.tile_waves == 0 ? p.head_units : hkv);
     const int most = p.tile_waves == 0 ? round / 2 : round;
     p.splits         = shared ? std::max(1, std::min(256, most / wgs)) : 0;
@@ -1048,10 +1088,12 @@ hipError_t launch_batch(uint16_t* out, int64_t out_stride, const uint16_t* q, in
 #define RTH_BATCH(W, G)                                                                        \
     batch_kernel<D, W, G><<<grid, block, 0, stream>>>(q, q_stride, t, own, plan, shared, p, pre, \
                                                       scale_log2)
-    if (p.tile_waves == 0) {
+    if (p.tile_waves == 0 && p.waves == 4) {
         RTH_BATCH(4, 0);
     } else if constexpr (D == 256) {
         RTH_BATCH(4, 1);
+    } else if (p.tile_waves == 0) {
+        RTH_BATCH(8, 0);
     } else if (p.tile_waves == 4) {
         RTH_BATCH(4, 2);
     } else {

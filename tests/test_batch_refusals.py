@@ -70,6 +70,7 @@ def test_append(change, says):
     (dict(so=100), "out_stride"), (dict(sq=4092), "q_stride"), (dict(tables=None), "block_tables"),
     (dict(width=-1), "table_blocks"), (dict(blocks=0), "num_blocks"), (dict(block=100), "power of two"),
     (dict(blocks=1 << 26), "2^31"), (dict(seqs=4096, hq=1 << 13, hkv=1, so=1 << 21, sq=1 << 21), "2^24"),
+    (dict(width=(1 << 28) + 1), "2^35"), (dict(seqs=4096, width=1 << 18), "2^35"),
 ])
 def test_decode(change, says):
     assert says in refuse("rth_attn_decode_batch", DECODE, **change)
