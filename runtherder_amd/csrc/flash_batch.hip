@@ -30,10 +30,10 @@
 //  * batch_merge_kernel joins the partials of a row.
 //
 // 32 q heads on 8, head_dim 128: 4 sequences behind 1000 shared keys 11 us (two
-// launches and the chain table -> page -> tile), 32 behind 8192 27 us (the same chain and
-// 21 MB), 128 behind 32768 105 us (69 GFLOP, 0.66 PFLOP/s; in the tile loop 0.99,
-// the rest is its start, the own keys and 35 MB of partials); 48 sequences of 100 to
-// 6000 own keys, head_dim 64, 35 us (bytes: 4.4 TB/s).
+// launches and the chain table -> page -> tile), 32 behind 8192 27 us (the same chain, four
+// rounds of tiles and 52 MB), 128 behind 32768 112 us (69 GFLOP, 0.62 PFLOP/s; in the tile
+// loop 0.9, the rest is its start, the own keys and 35 MB of partials); 48 sequences of 100 to
+// 6000 own keys, head_dim 64, 35 us (bytes: 4.5 TB/s).
 #include <algorithm>
 #include <type_traits>
 

@@ -20,9 +20,9 @@
 //    values, and the rows that do see such a value get it back at the end (1 to
 //    3 % of the time; a sequence must not hear what stands behind it).
 //
-// Bound by the matrix units: 16384 tokens, 32 q heads on 8, head_dim 128, 1.91 ms
-// = 1.15 PFLOP/s of the causal products, against 1.23 for a large matrix product.
-// Ragged prompts (12 of up to 1100 tokens, 88 us) pay beside that about 7 us a
+// Bound by the matrix units: 16384 tokens, 32 q heads on 8, head_dim 128, 1.95 to
+// 2.03 ms = 1.13 to 1.08 PFLOP/s of the causal products, against 1.38 for a large matrix
+// product. Ragged prompts (12 of 40 to 1100 tokens, 97 us) pay beside that about 7 us a
 // workgroup for its first tiles and the rows of q and out.
 #include <algorithm>
 #include <type_traits>

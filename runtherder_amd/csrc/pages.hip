@@ -12,9 +12,10 @@
 // 2 * (2 D + 8) per (row, kv head, layer); the bookkeeping by one read of refs
 // and the latency of its few steps.
 //
-// 8 kv heads, head_dim 128, pages of 64 keys: 48 pages of 32 layers copied in 67 us
-// (6.4 TB/s of reads and writes), a pool of 256 pages compacted in 105 us; a fork of 8
-// children, 15 us, is two launches and a chain of reads.
+// 8 kv heads, head_dim 128, pages of 64 keys: 48 pages of 32 layers copied in 81 us
+// (5.2 TB/s of reads and writes, a large copy's rate; 67 us where the last-level cache holds
+// some of them), a pool of 256 pages compacted in 119 us; freeing 8 children and forking 8,
+// 28 layers, 16 us: three launches and a chain of reads.
 #include <algorithm>
 
 #include "batch_common.hpp"
@@ -104,8 +105,8 @@ __device__ __forceinline__ void move_rows(const PageSlabs& s, const Move& m, int
     const int64_t  bytes = n * s.head_dim, n16 = bytes / 16;
     const int      tid = static_cast<int>(threadIdx.x);
     int64_t i = tid;
-    // Four loads on the way, and stores past the caches (48 pages of 32 layers, 428 MB
-    // read and written, 85 us; so 67, and with such loads as well 76).
+    // Four loads on the way, and stores past the caches (48 pages of 32 layers,
+    // the same ones each time, 85 us; so 67, and with such loads as well 76).
     for (; i + 3 * kMoveThr < n16; i += 4 * kMoveThr) {
         u32x4 x[4];
 #pragma unroll

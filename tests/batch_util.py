@@ -59,7 +59,8 @@ def score_size(q, k, scale):
 
 
 def quantize(x):
-    """(codes uint8, scale) of bf16 rows in the cache's format."""
+    """(codes uint8, scale) of bf16 rows in the cache's format. (448.0 / amax is a reciprocal times 448
+    here, so a code may lie a step from the append's at a tie.)"""
     x = x.float()
     amax = x.abs().amax(-1)
     inv = torch.where(amax > 0, 448.0 / amax, torch.zeros_like(amax))
