@@ -943,7 +943,7 @@ __global__ __launch_bounds__(batch_waves(kW, kG) * kWave, batch_per_simd(D, kW, 
 
 // ---- joining a row's partials ------------------------------------------------------
 
-// A workgroup joins the partials of a row: each group of D / 4 lanes (four floats a
+// A workgroup of kW waves joins the partials of a row: each group of D / 4 lanes (four floats a
 // lane) every kGroups-th one against a maximum of its own, four on the way
 // at a time, so that nothing waits for the maximum of all; then the groups.
 template <int D, int kW>

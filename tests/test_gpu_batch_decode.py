@@ -254,3 +254,38 @@ def test_graph_replays():
         t.attn.run_decode(out, q, view, lens, t.prefix_table, plen)   # eager work between
         sync()
         assert torch.equal(out, want)
+
+
+# Without a shared prefix; at head_dim 64 an odd kv head has no neighbour in its tile.
+@pytest.mark.parametrize("hq,hkv,d", [
+    (3, 3, 64), (9, 3, 64), (20, 1, 64), (35, 5, 64), (32, 8, 64), (6, 2, 64), (24, 8, 128), (7, 7, 128), (40, 2, 128),
+    (4, 2, 256),
+])
+def test_apart(hq, hkv, d):
+    t = Batch([300, 1, 77, 0, 140, 33, 1000], 0, hq, hkv, d, 32, 4000 + hq + d)
+    step(f"batch decode apart hq={hq} hkv={hkv} d={d}")
+    out = t.run(shared=False)
+    sync()
+    t.check(out.cpu())
+
+
+@pytest.mark.parametrize("hq,hkv", [(3, 3), (9, 3), (20, 1), (35, 5)])
+@pytest.mark.parametrize("own,prefix", [([30, 1, 77, 0, 140], 200), ([5, 40, 0, 65] * 20, 333)])
+def test_odd_heads_of_64(hq, hkv, own, prefix):
+    t = Batch(own, prefix, hq, hkv, 64, 64, 4300 + hq + len(own))
+    step(f"batch decode hq={hq} hkv={hkv} own={own[:5]}")
+    out = t.run()
+    sync()
+    t.check(out.cpu())
+
+
+# More rows than the merge's four waves a row fill the chip with; more sequences
+# than the bisection of the runs takes (its bound).
+@pytest.mark.parametrize("seqs,hq,hkv,d,prefix", [
+    (150, 16, 4, 128, 300), (150, 16, 4, 128, 0), (257, 8, 2, 64, 0), (256, 16, 2, 64, 100), (80, 32, 8, 256, 70)])
+def test_many_rows(seqs, hq, hkv, d, prefix):
+    t = Batch([(37 * i) % 190 for i in range(seqs)], prefix, hq, hkv, d, 32, 4500 + seqs + d)
+    step(f"batch decode {seqs} sequences hq={hq} d={d} prefix={prefix}")
+    out = t.run(shared=prefix > 0)
+    sync()
+    t.check(out.cpu())
