@@ -31,9 +31,17 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
+_ready = False   # the GPU was used (asked of torch once)
+
+
 def _current_device() -> int:
     """The current device; no tensor's where the GPU was never used."""
-    return _get_device() if torch.cuda.is_initialized() else -2
+    global _ready
+    if not _ready:
+        _ready = torch.cuda.is_initialized()
+        if not _ready:
+            return -2
+    return _get_device()
 
 
 def _stream(stream) -> int | None:
@@ -297,6 +305,13 @@ def rmsnorm_lanes(hidden_dim: int) -> int:
     return int(_ffi.load().rth_rmsnorm_lanes(hidden_dim))
 
 
+def _stream_of(stream, device: int) -> int | None:
+    """_stream, where the current device is known already."""
+    if stream is None and _raw_stream is not None:
+        return _raw_stream(device)
+    return _stream(stream)
+
+
 # ---- batches ---------------------------------------------------------------
 # No reference counterparts: the reference serves one sequence at a time.
 
@@ -311,18 +326,19 @@ def _need_on(t: torch.Tensor, dtype: torch.dtype, name: str, device: int) -> Non
         raise TypeError(f"{name} must be contiguous")
 
 
-def _need_rows(t: torch.Tensor, heads: int, head_dim: int, name: str, device: int) -> int:
+def _need_rows(t: torch.Tensor, rows: int, heads: int, head_dim: int, name: str,
+               device: int) -> int:
     """t: [rows, heads, head_dim] bf16, rows any stride apart; the stride."""
     if t.dtype != torch.bfloat16:
         raise TypeError(f"{name} must be torch.bfloat16, got {t.dtype}")
     if t.get_device() != device:
         raise TypeError(f"{name} must be a tensor of the current device")
-    shape, stride = t.shape, t.stride()
-    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim:
-        raise ValueError(f"{name} must be [rows, {heads}, {head_dim}], got {tuple(shape)}")
-    if stride[2] != 1 or (stride[1] != head_dim and heads > 1):
+    if t.shape != (rows, heads, head_dim):
+        raise ValueError(f"{name} must be [{rows}, {heads}, {head_dim}], got {tuple(t.shape)}")
+    row, head, one = t.stride()
+    if one != 1 or (head != head_dim and heads > 1):
         raise TypeError(f"{name}: a row's heads must be contiguous")
-    return stride[0] if shape[0] > 1 else heads * head_dim
+    return row if rows > 1 else heads * head_dim
 
 
 def _need_here(t: torch.Tensor, name: str, device: int) -> None:
@@ -365,18 +381,15 @@ def flash_packed_bf16(out, q, k, v, cu_seqlens, num_q_heads, num_kv_heads, head_
     cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of q, out [rows, Hq, D] and k, v
     [rows, Hkv, D] are sequence b. Rows may lie any stride apart (slices of a
     fused projection); rows behind the last sequence stay as they are."""
-    dev = _current_device()
-    so = _need_rows(out, num_q_heads, head_dim, "out", dev)
-    sq = _need_rows(q, num_q_heads, head_dim, "q", dev)
-    sk = _need_rows(k, num_kv_heads, head_dim, "k", dev)
-    sv = _need_rows(v, num_kv_heads, head_dim, "v", dev)
+    dev, n = _current_device(), len(q)
+    so = _need_rows(out, n, num_q_heads, head_dim, "out", dev)
+    sq = _need_rows(q, n, num_q_heads, head_dim, "q", dev)
+    sk = _need_rows(k, n, num_kv_heads, head_dim, "k", dev)
+    sv = _need_rows(v, n, num_kv_heads, head_dim, "v", dev)
     _need_on(cu_seqlens, torch.int32, "cu_seqlens", dev)
-    n = len(q)
-    if not len(out) == len(k) == len(v) == n:
-        raise ValueError("out, q, k and v must have the same number of rows")
     _ffi.call("rth_attn_packed", out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
               cu_seqlens.data_ptr(), cu_seqlens.numel() - 1, n, so, sq, sk, sv, num_q_heads,
-              num_kv_heads, head_dim, scale, _stream(stream))
+              num_kv_heads, head_dim, scale, _stream_of(stream, dev))
 
 
 def kv_append_fp8_batch(k_cache, v_cache, k_scale, v_scale, k, v, at_pos, block_tables,
@@ -385,21 +398,19 @@ def kv_append_fp8_batch(k_cache, v_cache, k_scale, v_scale, k, v, at_pos, block_
     one row per sequence) to the pages of their sequences, sequence b from
     position at_pos[b] on; bytes as PagedKVCache.append's. Rows without a page
     are not stored. Sequences that share a page do not both write to it."""
+    dev = _current_device()
     blocks = _need_slabs_of(k_cache, v_cache, k_scale, v_scale, block_size, num_kv_heads,
-                            head_dim, _current_device())
+                            head_dim, dev)
     _append_batch(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                   k, v, at_pos, block_tables, blocks, block_size, num_kv_heads, head_dim,
-                  cu_seqlens, stream)
+                  cu_seqlens, dev, stream)
 
 
 def _append_batch(kc, vc, ks, vs, k, v, at_pos, block_tables, num_blocks, block_size,
-                  num_kv_heads, head_dim, cu_seqlens, stream):
-    dev = _current_device()
-    sk = _need_rows(k, num_kv_heads, head_dim, "k", dev)
-    sv = _need_rows(v, num_kv_heads, head_dim, "v", dev)
+                  num_kv_heads, head_dim, cu_seqlens, dev, stream):
     n, seqs = len(k), at_pos.numel()
-    if len(v) != n:
-        raise ValueError("k and v must have the same number of rows")
+    sk = _need_rows(k, n, num_kv_heads, head_dim, "k", dev)
+    sv = _need_rows(v, n, num_kv_heads, head_dim, "v", dev)
     _need_on(at_pos, torch.int32, "at_pos", dev)
     if cu_seqlens is not None:
         _need_len(cu_seqlens, seqs + 1, "cu_seqlens", dev)
@@ -409,7 +420,7 @@ def _append_batch(kc, vc, ks, vs, k, v, at_pos, block_tables, num_blocks, block_
     width = _need_tables(block_tables, seqs, "block_tables", dev)
     _ffi.call("rth_kv_append_fp8_batch", kc, vc, ks, vs, k.data_ptr(), v.data_ptr(), sk, sv,
               cu_seqlens, at_pos.data_ptr(), seqs, n, num_kv_heads, head_dim,
-              block_tables.data_ptr(), width, num_blocks, block_size, _stream(stream))
+              block_tables.data_ptr(), width, num_blocks, block_size, _stream_of(stream, dev))
 
 
 def batch_scratch_floats(num_seqs: int, num_q_heads: int, num_kv_heads: int,
@@ -434,18 +445,14 @@ def flash_decode_batch_bf16(out, q, k, v, k_scale, v_scale, block_tables, block_
         raise ValueError("partial is smaller than batch_scratch_floats")
     _decode_batch(out, q, k, v, k_scale, v_scale, block_tables, width, blocks, block_size, lens,
                   partial, num_q_heads, num_kv_heads, head_dim, scale, prefix_table, prefix_len,
-                  stream)
+                  seqs, dev, stream)
 
 
 def _decode_batch(out, q, k, v, k_scale, v_scale, block_tables, width, num_blocks, block_size,
                   lens, partial, num_q_heads, num_kv_heads, head_dim, scale, prefix_table,
-                  prefix_len, stream):
-    dev = _current_device()
-    so = _need_rows(out, num_q_heads, head_dim, "out", dev)
-    sq = _need_rows(q, num_q_heads, head_dim, "q", dev)
-    seqs = len(q)
-    if len(out) != seqs:
-        raise ValueError("out and q must have the same number of rows")
+                  prefix_len, seqs, dev, stream):
+    so = _need_rows(out, seqs, num_q_heads, head_dim, "out", dev)
+    sq = _need_rows(q, seqs, num_q_heads, head_dim, "q", dev)
     _need_len(lens, seqs, "lens", dev)
     pt = pn = pl = 0
     if prefix_table is not None and prefix_len is not None:
@@ -457,7 +464,7 @@ def _decode_batch(out, q, k, v, k_scale, v_scale, block_tables, width, num_block
     _ffi.call("rth_attn_decode_batch", out.data_ptr(), so, q.data_ptr(), sq, k.data_ptr(),
               v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(), width,
               num_blocks, block_size, lens.data_ptr(), pt, pn, pl, partial.data_ptr(), seqs,
-              num_q_heads, num_kv_heads, head_dim, scale, _stream(stream))
+              num_q_heads, num_kv_heads, head_dim, scale, _stream_of(stream, dev))
 
 
 # ---- interface -------------------------------------------------------------
@@ -633,13 +640,14 @@ class PagedKVCache:
         (cu_seqlens), or one row per sequence, at at_pos[b] of sequence b."""
         if not 0 <= layer < self.num_layers:
             raise ValueError("KVCache append layer out of range")
-        _need_here(self.k, "the cache", _current_device())
+        dev = _current_device()
+        _need_here(self.k, "the cache", dev)
         rows = layer * self.num_blocks * self.block_size * self.num_kv_heads
         _append_batch(self.k.data_ptr() + rows * self.head_dim,
                       self.v.data_ptr() + rows * self.head_dim,
                       self.k_scale.data_ptr() + 4 * rows, self.v_scale.data_ptr() + 4 * rows, k, v,
                       at_pos, block_tables, self.num_blocks, self.block_size, self.num_kv_heads,
-                      self.head_dim, cu_seqlens, stream)
+                      self.head_dim, cu_seqlens, dev, stream)
 
     def batch_view(self, layer, block_tables) -> KVBatchView:
         if not 0 <= layer < self.num_layers:
@@ -666,7 +674,7 @@ class PagedKVCache:
         _need_len(dst, n, "dst", dev)
         if n:
             _ffi.call("rth_pages_copy", *self._all(), src.data_ptr(), dst.data_ptr(), n,
-                      _stream(stream))
+                      _stream_of(stream, dev))
 
 
 class PagePool:
@@ -704,7 +712,9 @@ class PagePool:
     def _of(self, cache):
         if cache.num_blocks != self.num_blocks or cache.block_size != self.block_size:
             raise ValueError("the pool and the cache differ in their blocks")
-        _need_here(cache.k, "the cache", self._here())
+        dev = self._here()
+        _need_here(cache.k, "the cache", dev)
+        return dev
 
     def reserve(self, block_tables, lens, n_new, stream=None):
         """Pages for positions lens[b] .. lens[b] + n_new[b] - 1 of sequence b,
@@ -716,7 +726,7 @@ class PagePool:
         _ffi.call("rth_pages_reserve", self.refs.data_ptr(), self._work.data_ptr(),
                   self.status.data_ptr(), self.num_blocks, self.block_size,
                   block_tables.data_ptr(), width, lens.data_ptr(), n_new.data_ptr(), seqs,
-                  _stream(stream))
+                  _stream_of(stream, dev))
 
     def fork(self, cache, dst_tables, dst_lens, src_tables, src_lens, parents, stream=None):
         """Sequence i of dst becomes a copy of sequence parents[i] of src (any
@@ -724,8 +734,7 @@ class PagePool:
         one): filled pages are shared, a part-filled last page is copied, in all
         layers of `cache`, into a page of the child's own. The dst tables hold no
         pages before (free them first)."""
-        self._of(cache)
-        dev, n, seqs = _current_device(), parents.numel(), src_lens.numel()
+        dev, n, seqs = self._of(cache), parents.numel(), src_lens.numel()
         _need_on(parents, torch.int32, "parents", dev)
         _need_on(src_lens, torch.int32, "src_lens", dev)
         _need_len(dst_lens, n, "dst_lens", dev)
@@ -735,7 +744,7 @@ class PagePool:
         _ffi.call("rth_pages_fork", *cache._all(), self.refs.data_ptr(), self._work.data_ptr(),
                   self.status.data_ptr(), dst_tables.data_ptr(), dst_lens.data_ptr(),
                   src_tables.data_ptr(), src_lens.data_ptr(), width, seqs, parents.data_ptr(), n,
-                  _stream(stream))
+                  _stream_of(stream, dev))
 
     def free(self, block_tables, lens, drop=None, stream=None):
         """Frees the sequences with drop[b] != 0 (None: all): their pages lose
@@ -747,17 +756,16 @@ class PagePool:
             _need_len(drop, seqs, "drop", dev)
             drop = drop.data_ptr()
         _ffi.call("rth_pages_free", self.refs.data_ptr(), self.num_blocks,
-                  block_tables.data_ptr(), width, lens.data_ptr(), drop, seqs, _stream(stream))
+                  block_tables.data_ptr(), width, lens.data_ptr(), drop, seqs, _stream_of(stream, dev))
 
     def compact(self, cache, block_tables, stream=None):
         """Moves the pages in use down to the lowest ones, in all layers of
         `cache`, and renames them in block_tables, which are all the tables that
         hold pages of the pool."""
-        self._of(cache)
-        seqs = len(block_tables)
-        width = _need_tables(block_tables, seqs, "block_tables", _current_device())
+        dev, seqs = self._of(cache), len(block_tables)
+        width = _need_tables(block_tables, seqs, "block_tables", dev)
         _ffi.call("rth_pages_compact", *cache._all(), self.refs.data_ptr(),
-                  self._work.data_ptr(), block_tables.data_ptr(), width, seqs, _stream(stream))
+                  self._work.data_ptr(), block_tables.data_ptr(), width, seqs, _stream_of(stream, dev))
 
 
 class AttentionBackend:
@@ -932,8 +940,6 @@ class BatchAttention:
         """flash_decode_batch_bf16 over kv with this object's scratch."""
         c, tables = self.config, kv.block_tables
         seqs, width = tables.shape
-        if len(q) != seqs:
-            raise ValueError(f"q holds {len(q)} sequences, the view {seqs}")
         if seqs > self.max_seqs:
             raise ValueError(f"{seqs} sequences: this backend was made for {self.max_seqs}")
         if kv.num_kv_heads != c.num_kv_heads or kv.head_dim != c.head_dim:
@@ -942,7 +948,7 @@ class BatchAttention:
         _need_here(kv.k, "the view", dev); _need_here(self.partial, "the scratch", dev)
         _decode_batch(out, q, kv.k, kv.v, kv.k_scale, kv.v_scale, tables, width, kv.num_blocks,
                       kv.block_size, lens, self.partial, c.num_q_heads, c.num_kv_heads, c.head_dim,
-                      c.scale, prefix_table, prefix_len, stream)
+                      c.scale, prefix_table, prefix_len, seqs, dev, stream)
 
 
 class NaiveAttention(AttentionBackend):
