@@ -29,7 +29,7 @@
 //    the bf16 MFMA; the row sum takes the fp32 weights.
 //  * batch_merge_kernel joins the partials of a row.
 //
-// 32 q heads on 8, head_dim 128: 4 sequences behind 1000 shared keys 11 us (two
+// 32 q heads on 8, head_dim 128: 4 sequences behind 1000 shared keys 10 us (two
 // launches and the chain table -> page -> tile), 32 behind 8192 27 us (the same chain, four
 // rounds of tiles and 52 MB), 128 behind 32768 112 us (69 GFLOP, 0.62 PFLOP/s; in the tile
 // loop 0.9, the rest is its start, the own keys and 35 MB of partials); 48 sequences of 100 to
