@@ -86,6 +86,37 @@ __device__ __forceinline__ bool find_block(int w, int num_seqs, F blocks, BlockO
     return false;
 }
 
+// The same for up to a wave of sequences (lane b: n blocks): each lane sums for an index of
+// its own (one prompt of 200 tokens, against one index after the other, 10.8 -> 10.2 us;
+// 30 ragged ones 165 -> 166).
+__device__ __forceinline__ bool find_block_of_wave(int w, int num_seqs, int n, int lane, BlockOf& at) {
+    int step = 1;
+    while (__any(n > step * kWave)) {
+        step *= kWave;
+    }
+    int lo = 0, above = 0;
+    for (;; step /= kWave) {
+        const int t = lo + lane * step;
+        int       from = 0;   // blocks with index >= t
+        for (int b = 0; b < num_seqs; ++b) {
+            from += max(0, __builtin_amdgcn_readlane(n, b) - t);
+        }
+        const int over = __popcll(__ballot(from > w));   // (from falls with t)
+        if (over == 0) {
+            return false;
+        }
+        above = over < kWave ? __builtin_amdgcn_readlane(from, over) : above;
+        lo += (over - 1) * step;
+        if (step == 1) {
+            break;
+        }
+    }
+    const bool     mine = n > lo;
+    const uint64_t hit  = __ballot(mine && lanes_below(__ballot(mine)) == w - above);
+    at = {__ffsll(static_cast<unsigned long long>(hit)) - 1, lo};
+    return true;
+}
+
 template <int D, int kW>   // kW waves of 32 rows
 __global__ __launch_bounds__(kW * kWave, D < 256 ? 2 : 1) void flash_packed_kernel(
     uint16_t* __restrict__ out, const uint16_t* __restrict__ q, const uint16_t* __restrict__ k,
@@ -114,34 +145,39 @@ __global__ __launch_bounds__(kW * kWave, D < 256 ? 2 : 1) void flash_packed_kern
     const int kvh = (hkv & 7) == 0 ? (hb & 7) * (hkv >> 3) + (hb >> 3) : hb;
 
     BlockOf at;
-    bool    found;
+    int     first, n;   // the sequence's rows
     {
-        auto count = [&](int b) {
-            const int n = b < num_seqs
-                              ? clamp_rows(cu[b + 1], num_rows) - clamp_rows(cu[b], num_rows) : 0;
-            return static_cast<int>((static_cast<int64_t>(max(n, 0)) * group + kBM - 1) / kBM);
+        auto bound = [&](int b) { return b <= num_seqs ? clamp_rows(cu[b], num_rows) : 0; };
+        auto count = [&](int rows) {
+            return static_cast<int>((static_cast<int64_t>(max(rows, 0)) * group + kBM - 1) / kBM);
         };
+        bool found;
         if (num_seqs <= kWave) {   // every wave by itself, from registers
-            const int n = count(lane);
-            found       = find_block(w, num_seqs, [&](int) { return n; }, at);
+            const int from = bound(lane), to = bound(lane + 1);
+            found = find_block_of_wave(w, num_seqs, lane < num_seqs ? count(to - from) : 0, lane, at);
+            if (found) {
+                first = __builtin_amdgcn_readlane(from, uniform(at.seq));
+                n     = __builtin_amdgcn_readlane(to, uniform(at.seq)) - first;
+            }
         } else {
             int* nblk = reinterpret_cast<int*>(lds);
             for (int b = tid; b < num_seqs; b += kThr) {
-                nblk[b] = count(b);
+                nblk[b] = count(bound(b + 1) - bound(b));
             }
             __syncthreads();
             found = find_block(
                 w, num_seqs, [&](int b0) { return b0 + lane < num_seqs ? nblk[b0 + lane] : 0; }, at);
             __syncthreads();
+            if (found) {
+                first = uniform(bound(at.seq));
+                n     = uniform(bound(at.seq + 1)) - first;
+            }
         }
         if (!found) {
             return;
         }
     }
-    const int seq   = __builtin_amdgcn_readfirstlane(at.seq);
     const int j     = __builtin_amdgcn_readfirstlane(at.j);
-    const int first = clamp_rows(cu[seq], num_rows);
-    const int n     = clamp_rows(cu[seq + 1], num_rows) - first;
     const int rows  = n * group;
     const int r0    = j * kBM;
     const int n_tiles = (min(r0 + kBM, rows) - 1) / group / T::kN + 1;
