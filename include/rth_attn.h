@@ -383,8 +383,9 @@ int rth_kv_append_fp8_batch(uint8_t* k_cache, uint8_t* v_cache, float* k_scale, 
  * (so tables that rth_pages_fork made can be passed whole, with any one of
  * their rows as prefix_table). prefix_table and prefix_len NULL: nothing is shared. lens[b] <= 0:
  * an unused slot, its output row is zeros. A sequence shorter than the prefix sees
- * its lens[b] keys of it (where the others are finite: the rows of a kv head are one
- * product, in which a NaN or an infinity times a weight of 0 is a NaN). Keys past a table's end, and keys whose
+ * its lens[b] keys of it (where those that a longer one sees are finite: the rows of a kv head
+ * are one product, in which a NaN or an infinity times a weight of 0 is a NaN; what no
+ * sequence sees does not matter). Keys past a table's end, and keys whose
  * table entry names no page, are left out. head_dim 64, 128, 256; any Hq / Hkv;
  * num_seqs * Hq <= 2^24, num_seqs * table_blocks * block_size <= 2^35.
  * partial: rth_batch_scratch_floats floats, 16-byte aligned, no

@@ -39,6 +39,20 @@ __device__ __forceinline__ int wave_sum_i(int v) {
     return static_cast<int>(b[0] + b[1]);
 }
 
+// Maximum over the wave, likewise.
+__device__ __forceinline__ int wave_max_i(int v) {
+    v = max(v, dpp_i<0xB1>(v));
+    v = max(v, dpp_i<0x4E>(v));
+    v = max(v, dpp_i<0x141>(v));
+    v = max(v, dpp_i<0x140>(v));
+    const auto a = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(v),
+                                                    static_cast<uint32_t>(v), false, false);
+    v            = max(static_cast<int>(a[0]), static_cast<int>(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(v),
+                                                    static_cast<uint32_t>(v), false, false);
+    return max(static_cast<int>(b[0]), static_cast<int>(b[1]));
+}
+
 // Set bits of `mask` below this lane.
 __device__ __forceinline__ int lanes_below(uint64_t mask) {
     return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),

@@ -73,6 +73,19 @@ __device__ __forceinline__ int prefix_keys(const BatchView& t) {
 
 constexpr int kHalf = 32;   // keys of one score block
 
+// How many of the prefix's keys some sequence sees. The others may never have
+// been written, and a weight of 0 takes a NaN from them: they are not read.
+__device__ __forceinline__ int prefix_seen(const BatchView& t, int prefix, int lane) {
+    int n = 0;
+    for (int b0 = 0; b0 < t.num_seqs; b0 += 4 * kWave) {   // four loads on the way
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            n = max(n, t.lens[min(b0 + i * kWave + lane, t.num_seqs - 1)]);
+        }
+    }
+    return min(prefix, uniform(wave_max_i(n)));
+}
+
 // Keys [from, to) of a run of tiles of n keys.
 struct Keys {
     int from, to;
@@ -527,8 +540,8 @@ __device__ __forceinline__ void prefix_units(uint8_t* lds, int bid, int prefix,
     WaveRows<D> w(t, lds + wave * T::kBytes, lane, kvh, scale_log2);
     w.load_q(q + b * q_stride + static_cast<int64_t>(head) * D, t.group * D);
     const int first = split * runs.per;
-    w.run(t.prefix_table, Keys{0, prefix}, first + wave, min(first + runs.per, tiles), kW,
-          t.lens[b]);
+    w.run(t.prefix_table, Keys{0, prefix_seen(t, prefix, lane)}, first + wave, min(first + runs.per, tiles),
+          kW, t.lens[b]);
     const int64_t all = static_cast<int64_t>(bp.splits) * t.num_seqs * hq;
     float m[T::kHeads], l[T::kHeads];
 #pragma unroll
@@ -674,6 +687,8 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D> (&sm)[kG], int bid, in
     const int tile0     = split * runs.per + group * rounds;
     const int n_tiles   = min(rounds, all_tiles - group * rounds);
 
+    int seen_to = prefix;   // (found out below, while the first table entries are on the way)
+
     // A thread copies 16 codes of a row in each copy step; the rows of a wave
     // lie in one half of the tile, so in one page, and their base is scalar.
     constexpr int kWaveRows = kWave / kCpr;
@@ -702,11 +717,11 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D> (&sm)[kG], int bid, in
     auto pages = [&](int i, const Entries& e) {
         const int key = (tile0 + i) * T::kN, lo = uniform(e.lo), hi = uniform(e.hi);
         return Pages{t.row(t.is_page(lo) ? lo : 0, key), t.row(t.is_page(hi) ? hi : 0, key + kHalf),
-                     (t.is_page(lo) ? 1 : 0) | (t.is_page(hi) ? 2 : 0)};
+                     (t.is_page(lo) && key < seen_to ? 1 : 0) | (t.is_page(hi) && key + kHalf < seen_to ? 2 : 0)};
     };
-    // The row of half u that row r of it reads: past the prefix, its last one.
+    // The row of half u that row r of it reads: past the keys that are seen, the last one.
     auto row_of = [&](int i, int u, int r) {
-        return static_cast<uint32_t>(min(r, max(prefix - 1 - (tile0 + i) * T::kN - u * kHalf, 0)));
+        return static_cast<uint32_t>(min(r, max(seen_to - 1 - (tile0 + i) * T::kN - u * kHalf, 0)));
     };
     auto load = [&](const uint8_t* x, int i, const Pages& p, u32x4 (&reg)[kSteps]) {
         const int tt = again(tid), crow = tt / kCpr, cchunk = tt % kCpr;   // (computed anew: registers)
@@ -751,8 +766,10 @@ __device__ __forceinline__ void prefix_tiles(PrefixLds<D> (&sm)[kG], int bid, in
     };
 
     // pa, pb: pages of tiles i and i + 1 (at iteration i), e2, e3: entries of the two after.
-    Pages   pa = pages(0, entries(0)), pb = pages(1, entries(1));
-    Entries e2 = entries(2), e3 = entries(3);
+    const Entries e0 = entries(0), e1 = entries(1);
+    Entries       e2 = entries(2), e3 = entries(3);
+    seen_to  = prefix_seen(t, prefix, lane);
+    Pages pa = pages(0, e0), pb = pages(1, e1);
     if (n_tiles > 0) {
         load(t.k, 0, pa, kreg);
         load_fac(0, pa);

@@ -214,3 +214,71 @@ def test_cpp_batch_driver():
     print(res.stdout[-4000:], res.stderr[-2000:])
     assert res.returncode == 0
     assert "ALL OK" in res.stdout
+
+
+def test_a_captured_decode_takes_the_prefix_as_it_is():
+    """The prefix's length lives on the device: replays with other lengths of it, from none
+    to the whole prompt, give what the eager calls give; the keys are the same ones, so
+    all agree within the outputs' bounds."""
+    s = Serving(3, 1, 64, 64, 16, 16, 4, 128)
+    step("captured decode, prefix lengths")
+    s.prompts([600, 0, 0])
+    tables, lens = s.pool.new_tables(20, 16), ints([0] * 20)
+    s.pool.fork(s.cache, tables, lens, s.tables, s.lens, ints([0] * 20))
+    s.rows = [list(s.rows[0]) for _ in range(20)]
+    q = s.draw(1, 20, 16, 128)
+    dq, out, plen = q[0].to(DEV), torch.zeros((20, 16, 128), dtype=torch.bfloat16, device=DEV), ints([64])
+    view = s.cache.batch_view(0, tables)
+
+    def run():
+        s.attn.run_decode(out, dq, view, lens, tables[3], plen)
+
+    run()
+    sync()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for n in (0, 1, 64, 300, 576, 600, 5000, 0):
+        plen.fill_(n)
+        got = []
+        for call in (run, graph.replay):
+            out.zero_()
+            call()
+            sync()
+            got.append(out.clone())
+        assert torch.equal(*got), n
+        s.check(q, got[0][None])   # (what lies behind the 600 keys was never written)
+
+
+def test_two_streams_at_once():
+    """Calls that overlap, each with a scratch of its own, over one cache."""
+    s = Serving(6, 1, 64, 64, 16, 32, 8, 128)
+    step("two streams")
+    s.prompts([500, 33, 800, 64, 1, 250])
+    q = [s.draw(6, 32, 128).to(DEV) for _ in range(8)]
+    k, v = (s.draw(1649, 8, 128).to(DEV) for _ in range(2))
+    qp, cu = s.draw(1649, 32, 128).to(DEV), ints(cu_of([1000, 249, 400]))
+    view = s.cache.batch_view(0, s.tables)
+    attns = [R.BatchAttention(R.AttnConfig(32, 8, 128, s.scale), 6, device=DEV) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    want = []
+    for x in q:
+        o = torch.empty_like(x)
+        attns[0].run_decode(o, x, view, s.lens)
+        want.append(o)
+    wp = torch.empty_like(qp)
+    attns[0].run_packed(wp, qp, k, v, cu)
+    sync()
+    outs = [[torch.zeros_like(x) for x in q] for _ in range(2)]
+    packed = [torch.zeros_like(qp) for _ in range(2)]
+    sync()
+    for i, x in enumerate(q):
+        for j in range(2):
+            attns[j].run_decode(outs[j][i], x, view, s.lens, stream=streams[j])
+            if i == 3 + j:
+                attns[j].run_packed(packed[j], qp, k, v, cu, stream=streams[j])
+    sync()
+    for j in range(2):
+        assert torch.equal(packed[j], wp)
+        for a, b in zip(outs[j], want):
+            assert torch.equal(a, b)
